@@ -19,7 +19,7 @@ LIBRARY = os.path.join(HERE, "libfunasr_hip.so")
 # batcher (no HIP code; built with the host compiler).
 BENCH_WORKERS = os.path.join(HERE, "libfah_bench_workers.so")
 SOURCES = ["fah_kernels.hip", "fah_persistent.hip", "fah_prefill.hip", "fah_sessions.hip", "fah_float.hip",
-           "fah_api.hip"]
+           "fah_attention.hip", "fah_choice.hip", "fah_api.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
          "-fno-gpu-flush-denormals-to-zero", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

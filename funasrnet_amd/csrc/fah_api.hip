@@ -13,6 +13,7 @@
 #include <condition_variable>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <memory>
 #include <mutex>
 #include <optional>
@@ -2112,6 +2113,159 @@ int fah_q8_block_dots_device(fah_context* h, const int8_t* q, const fah_weight* 
     DeviceWork work(*c);
     check(fah::launch_block_dots(q, w->q.as<int8_t>(), w->rows, w->cols, dots, c->stream), "block dots");
     return FAH_OK;
+  });
+}
+
+// Serving operators: stateless calls on the caller's descriptor, ordered on the
+// context stream.
+}  // extern "C"
+
+namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Element strides of a type whose byte strides are multiples of 16, and not negative.
+bool strides16(int type, std::initializer_list<int64_t> strides) {
+  for (int64_t n : strides)
+    if (n < 0 || n % (type == FAH_TYPE_F32 ? 4 : 8) != 0) return false;
+  return true;
+}
+
+void require_workspace(const void* p, int64_t have, int64_t need) {
+  require(need == 0 || (p && have >= need && aligned16(p)),
+          "the workspace needs " + std::to_string(need) + " bytes at a 16-byte boundary");
+}
+
+// False: declined.
+bool check_packed(const fah_packed_attention& a) {
+  require(a.sequences >= 0 && a.query_rows >= 0 && a.key_rows >= 0 && a.longest_query >= 0 && a.longest_key >= 0,
+          "negative attention sizes");
+  require(a.heads > 0 && a.kv_heads > 0 && a.head_size > 0 && a.heads % a.kv_heads == 0,
+          "heads must be a multiple of the K/V heads");
+  require(std::isfinite(a.scale) && a.scale > 0, "the attention scale must be above 0");
+  require((int64_t)a.query_rows * a.heads <= INT32_MAX / 2 && (int64_t)a.sequences * a.heads <= INT32_MAX / 256,
+          "too many query rows or sequences");
+  return fah::attention_supported(a.heads, a.kv_heads, a.head_size, a.query_type, a.cache_type) &&
+         strides16(a.query_type, {a.query_row, a.query_head, a.output_row, a.output_head}) &&
+         strides16(a.cache_type, {a.key_row, a.key_head, a.value_row, a.value_head});
+}
+
+bool check_prefix(const fah_prefix_attention& a) {
+  require(a.sequences >= 0 && a.prefix >= 0 && a.capacity >= 0 && a.longest >= 0, "negative attention sizes");
+  require(a.heads > 0 && a.kv_heads > 0 && a.head_size > 0 && a.heads % a.kv_heads == 0,
+          "heads must be a multiple of the K/V heads");
+  require(std::isfinite(a.scale) && a.scale > 0, "the attention scale must be above 0");
+  require((int64_t)a.sequences * a.heads <= INT32_MAX / 256, "too many sequences");
+  return fah::attention_supported(a.heads, a.kv_heads, a.head_size, a.query_type, a.cache_type) &&
+         strides16(a.query_type, {a.query_sequence, a.query_head, a.output_sequence, a.output_head}) &&
+         strides16(a.cache_type, {a.prefix_key_row, a.prefix_key_head, a.prefix_value_row, a.prefix_value_head,
+                                  a.key_sequence, a.key_row, a.key_head, a.value_sequence, a.value_row, a.value_head});
+}
+
+bool check_logits(const fah_logits_adjust& a) {
+  require(a.rows >= 0 && a.vocab >= 0 && a.history_capacity >= 0 && a.bias_capacity >= 0 && a.mask_rows >= 0,
+          "negative logits sizes");
+  require(a.rows <= 65535, "more than 65535 rows of logits");
+  require(a.vocab <= INT32_MAX / 2, "too many tokens");
+  return a.type == FAH_TYPE_F32 || a.type == FAH_TYPE_F16 || a.type == FAH_TYPE_BF16;
+}
+
+// One serving call: `run` enqueues on the context stream.
+template <typename F>
+int serve(fah_context* h, const void* call, F&& run) {
+  if (!h) return fail(FAH_ERROR_ARGUMENT, "context is NULL");
+  if (!call) return fail(FAH_ERROR_ARGUMENT, "call is NULL");
+  Ctx* c = h->st.get();
+  return guarded([&]() -> int { return run(c); });
+}
+
+// The enqueue section of a serving call.
+template <typename F>
+int enqueue(Ctx* c, const char* what, F&& launch) {
+  std::lock_guard<std::mutex> lock(c->gate);
+  if (c->disposed) return fail(FAH_ERROR_DISPOSED, "context disposed");
+  check(hipSetDevice(c->device), "hipSetDevice");
+  DeviceWork work(*c);
+  check(launch(c->stream), what);
+  return FAH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fah_attention_packed_workspace(const fah_packed_attention* a, int64_t* bytes) {
+  return guarded([&]() -> int {
+    require(a && bytes, "call/bytes is NULL");
+    if (!check_packed(*a)) return FAH_DECLINED;
+    *bytes = fah::packed_attention_workspace(*a);
+    return FAH_OK;
+  });
+}
+
+int fah_attention_packed_device(fah_context* h, const fah_packed_attention* a) {
+  return serve(h, a, [&](Ctx* c) {
+    if (!check_packed(*a)) return FAH_DECLINED;
+    if (a->sequences == 0 || a->query_rows == 0) return FAH_OK;
+    require(a->query && a->output && a->query_offsets && (a->key_rows == 0 || (a->key && a->value)),
+            "NULL attention buffer");
+    if (!aligned16(a->query) || !aligned16(a->key) || !aligned16(a->value) || !aligned16(a->output)) return FAH_DECLINED;
+    require_workspace(a->workspace, a->workspace_bytes, fah::packed_attention_workspace(*a));
+    return enqueue(c, "packed attention", [&](hipStream_t s) { return fah::launch_packed_attention(*a, s); });
+  });
+}
+
+int fah_attention_prefix_workspace(const fah_prefix_attention* a, int64_t* bytes) {
+  return guarded([&]() -> int {
+    require(a && bytes, "call/bytes is NULL");
+    if (!check_prefix(*a)) return FAH_DECLINED;
+    *bytes = fah::prefix_attention_workspace(*a);
+    return FAH_OK;
+  });
+}
+
+int fah_attention_prefix_device(fah_context* h, const fah_prefix_attention* a) {
+  return serve(h, a, [&](Ctx* c) {
+    if (!check_prefix(*a)) return FAH_DECLINED;
+    if (a->sequences == 0) return FAH_OK;
+    require(a->query && a->output && a->lengths && (a->prefix == 0 || (a->prefix_key && a->prefix_value)) &&
+                (a->capacity == 0 || (a->key && a->value)),
+            "NULL attention buffer");
+    if (!aligned16(a->query) || !aligned16(a->prefix_key) || !aligned16(a->prefix_value) || !aligned16(a->key) ||
+        !aligned16(a->value) || !aligned16(a->output))
+      return FAH_DECLINED;
+    require_workspace(a->workspace, a->workspace_bytes, fah::prefix_attention_workspace(*a));
+    return enqueue(c, "prefix attention", [&](hipStream_t s) { return fah::launch_prefix_attention(*a, s); });
+  });
+}
+
+int fah_logits_adjust_workspace(const fah_logits_adjust* a, int64_t* bytes) {
+  return guarded([&]() -> int {
+    require(a && bytes, "call/bytes is NULL");
+    if (!check_logits(*a)) return FAH_DECLINED;
+    *bytes = fah::logits_adjust_workspace(*a);
+    return FAH_OK;
+  });
+}
+
+int fah_logits_adjust_device(fah_context* h, const fah_logits_adjust* a) {
+  return serve(h, a, [&](Ctx* c) {
+    if (!check_logits(*a)) return FAH_DECLINED;
+    if (a->rows == 0) return FAH_OK;
+    const uintptr_t element = a->type == FAH_TYPE_F32 ? 4 : 2;
+    require(a->vocab > 0 && a->logits && a->output, "logits need an input, an output and a vocabulary");
+    require(reinterpret_cast<uintptr_t>(a->logits) % element == 0 && reinterpret_cast<uintptr_t>(a->output) % element == 0,
+            "logits must start on a whole element");
+    require(a->rows == 1 || (a->logits_stride >= 0 && a->output_stride >= a->vocab), "invalid logits strides");
+    require(a->logits != a->output || a->rows == 1 || a->logits_stride == a->output_stride,
+            "logits in place need one stride");
+    require(a->history_capacity == 0 || (a->history && a->history_stride >= 0), "invalid history");
+    require(a->bias_capacity == 0 || (a->bias_tokens && a->bias_values && a->bias_stride >= 0), "invalid biases");
+    require(a->mask_rows == 0 || (a->masks && a->mask_stride >= (a->mask_rows > 1 ? (a->vocab + 31) / 32 : 0)),
+            "invalid masks");
+    require(a->mask_rows <= 1 || a->mask_index || a->mask_rows >= a->rows, "fewer masks than rows need an index");
+    require_workspace(a->workspace, a->workspace_bytes, fah::logits_adjust_workspace(*a));
+    return enqueue(c, "logits", [&](hipStream_t s) { return fah::launch_logits_adjust(*a, s); });
   });
 }
 

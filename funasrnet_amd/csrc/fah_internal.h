@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "../../include/funasr_hip.h"
+
 namespace fah {
 
 enum InputMode { kInputQuantized = 0, kInputFloat = 1, kInputNorm = 2 };
@@ -319,6 +321,17 @@ int session_step_positions();
 int session_step_groups();
 int session_step_blocks_per_cu(int width);
 hipError_t launch_session_step(const SessionStepArgs& a, hipStream_t s);
+
+// Serving operators (fah_attention.hip, fah_choice.hip): the descriptors of the
+// C ABI, checked by the caller (attention_supported; every size at least 0).
+// The *_workspace functions read no pointer of theirs.
+bool attention_supported(int heads, int kv_heads, int head_size, int query_type, int cache_type);
+int64_t packed_attention_workspace(const fah_packed_attention& a);
+hipError_t launch_packed_attention(const fah_packed_attention& a, hipStream_t s);
+int64_t prefix_attention_workspace(const fah_prefix_attention& a);
+hipError_t launch_prefix_attention(const fah_prefix_attention& a, hipStream_t s);
+int64_t logits_adjust_workspace(const fah_logits_adjust& a);
+hipError_t launch_logits_adjust(const fah_logits_adjust& a, hipStream_t s);
 
 int gemv_max_k();
 int gemv_pairs_per_thread(int group_rows, int K);

@@ -34,6 +34,7 @@ _f32p = ctypes.POINTER(ctypes.c_float)
 _i8p = ctypes.POINTER(ctypes.c_int8)
 _i32p = ctypes.POINTER(ctypes.c_int32)
 _u16p = ctypes.POINTER(ctypes.c_uint16)
+_i64p = ctypes.POINTER(ctypes.c_int64)
 
 
 class Q8Host(ctypes.Structure):
@@ -56,6 +57,45 @@ class CallStats(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int64) for n in ("calls", "declined", "operations", "uploaded_bytes",
                                                "downloaded_bytes")] + [
         ("device_ms", ctypes.c_double), ("total_ms", ctypes.c_double)]
+
+
+# Element types (FAH_TYPE_*).
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+
+
+class PackedAttention(ctypes.Structure):
+    """fah_packed_attention: pointers are integers (e.g. torch data_ptr()), strides count elements."""
+    _fields_ = [(n, _vp) for n in ("query", "key", "value", "output")] + [
+        (n, ctypes.c_int64) for n in ("query_row", "query_head", "key_row", "key_head", "value_row", "value_head",
+                                      "output_row", "output_head")] + [
+        (n, _vp) for n in ("query_offsets", "key_offsets")] + [
+        (n, ctypes.c_int) for n in ("sequences", "query_rows", "key_rows", "longest_query", "longest_key", "heads",
+                                    "kv_heads", "head_size", "query_type", "cache_type")] + [
+        ("scale", ctypes.c_float), ("workspace", _vp), ("workspace_bytes", ctypes.c_int64)]
+
+
+class PrefixAttention(ctypes.Structure):
+    """fah_prefix_attention, as PackedAttention."""
+    _fields_ = [(n, _vp) for n in ("query", "prefix_key", "prefix_value", "key", "value", "output", "lengths")] + [
+        (n, ctypes.c_int64) for n in ("query_sequence", "query_head", "prefix_key_row", "prefix_key_head",
+                                      "prefix_value_row", "prefix_value_head", "key_sequence", "key_row", "key_head",
+                                      "value_sequence", "value_row", "value_head", "output_sequence", "output_head")] + [
+        (n, ctypes.c_int) for n in ("sequences", "prefix", "capacity", "longest", "heads", "kv_heads", "head_size",
+                                    "query_type", "cache_type")] + [
+        ("scale", ctypes.c_float), ("workspace", _vp), ("workspace_bytes", ctypes.c_int64)]
+
+
+class LogitsAdjust(ctypes.Structure):
+    """fah_logits_adjust, as PackedAttention."""
+    _fields_ = [(n, _vp) for n in ("logits", "output", "tokens")] + [
+        (n, ctypes.c_int64) for n in ("logits_stride", "output_stride")] + [
+        (n, ctypes.c_int) for n in ("rows", "vocab", "type", "history_capacity")] + [
+        ("history", _vp), ("history_stride", ctypes.c_int64)] + [
+        (n, _vp) for n in ("history_counts", "prompt_counts", "repetition", "presence", "frequency", "bias_tokens",
+                           "bias_values")] + [
+        ("bias_stride", ctypes.c_int64), ("bias_capacity", ctypes.c_int), ("mask_rows", ctypes.c_int),
+        ("bias_counts", _vp), ("masks", _vp), ("mask_stride", ctypes.c_int64), ("mask_index", _vp), ("workspace", _vp),
+        ("workspace_bytes", ctypes.c_int64)]
 
 
 # Seam entry points in fah_context_statistics order (FAH_CALL_*).
@@ -96,6 +136,12 @@ SIGNATURES = {
     "fah_q8_block_dots_device": (ctypes.c_int, [_vp, _vp, _vp, _vp]),
     "fah_linear_device": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, _vp, _vp]),
     "fah_attention_device": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp]),
+    "fah_attention_packed_device": (ctypes.c_int, [_vp, ctypes.POINTER(PackedAttention)]),
+    "fah_attention_packed_workspace": (ctypes.c_int, [ctypes.POINTER(PackedAttention), _i64p]),
+    "fah_attention_prefix_device": (ctypes.c_int, [_vp, ctypes.POINTER(PrefixAttention)]),
+    "fah_attention_prefix_workspace": (ctypes.c_int, [ctypes.POINTER(PrefixAttention), _i64p]),
+    "fah_logits_adjust_device": (ctypes.c_int, [_vp, ctypes.POINTER(LogitsAdjust)]),
+    "fah_logits_adjust_workspace": (ctypes.c_int, [ctypes.POINTER(LogitsAdjust), _i64p]),
     "fah_decoder_create": (ctypes.c_int, [_vp, ctypes.POINTER(DecoderConfigC), ctypes.POINTER(LayerHost),
                                           ctypes.POINTER(Q8Host), ctypes.POINTER(Q8Host), _f32p,
                                           ctypes.POINTER(_vp)]),
@@ -399,6 +445,34 @@ class HipBackend:
     def attention_device(self, q_ptr: int, k_ptr: int, v_ptr: int, frames: int, width: int, heads: int,
                          out_ptr: int) -> int:
         return _check(load().fah_attention_device(self.handle, q_ptr, k_ptr, v_ptr, frames, width, heads, out_ptr))
+
+    # serving operators: a descriptor (kept from call to call if its fields stay) and its workspace
+    def _workspace(self, name: str, call) -> int:
+        """Bytes; 0 too for calls that the library declines."""
+        v = ctypes.c_int64()
+        _check(getattr(load(), name)(ctypes.byref(call), ctypes.byref(v)))
+        return v.value
+
+    def attention_packed_workspace(self, call: PackedAttention) -> int:
+        return self._workspace("fah_attention_packed_workspace", call)
+
+    def attention_packed_device(self, call: PackedAttention) -> int:
+        """Causal attention over packed prompts (fah_attention_packed_device)."""
+        return _check(load().fah_attention_packed_device(self.handle, ctypes.byref(call)))
+
+    def attention_prefix_workspace(self, call: PrefixAttention) -> int:
+        return self._workspace("fah_attention_prefix_workspace", call)
+
+    def attention_prefix_device(self, call: PrefixAttention) -> int:
+        """One token a sequence over a shared prefix and own cache rows (fah_attention_prefix_device)."""
+        return _check(load().fah_attention_prefix_device(self.handle, ctypes.byref(call)))
+
+    def logits_adjust_workspace(self, call: LogitsAdjust) -> int:
+        return self._workspace("fah_logits_adjust_workspace", call)
+
+    def logits_adjust_device(self, call: LogitsAdjust) -> int:
+        """Penalties, biases and masks on logits, and the greedy choice after them (fah_logits_adjust_device)."""
+        return _check(load().fah_logits_adjust_device(self.handle, ctypes.byref(call)))
 
     def block_dots_device(self, q_ptr: int, weight: HipWeight, dots_ptr: int):
         _check(load().fah_q8_block_dots_device(self.handle, q_ptr, weight.handle, dots_ptr))

@@ -258,6 +258,133 @@ int fah_attention_device(fah_context* context, const float* query, const float* 
  * TensorMath.QuantizedRowsAvx.cs:80-87), for bit-exact verification. */
 int fah_q8_block_dots_device(fah_context* context, const int8_t* q, const fah_weight* weight, int32_t* dots);
 
+/* Serving operators (device-resident buffers) --------------------------------
+ * What a batch of recordings needs beside the decoder's own steps: attention
+ * over several prompts in one call, decoding behind a prompt prefix that all
+ * of them share, and the choice of a token under penalties, biases and masks.
+ *
+ * The descriptors' pointers are device addresses on the context's device, and
+ * their strides count elements. Work is ordered on the context stream (order
+ * other streams with it through fah_context_stream and events); the calls
+ * copy nothing, wait for nothing, allocate nothing and keep nothing, so they
+ * may be captured into graphs. What they need beyond their outputs is the
+ * caller's `workspace`: at least the bytes that the *_workspace call of the
+ * same descriptor gives (it needs no device and reads nothing through the
+ * pointers), 16-byte aligned, its contents free before and after. Calls that may run at the same time, such as two
+ * graphs replayed on different streams, need workspaces of their own.
+ * No output may overlap an input or the workspace unless its comment says so. */
+
+/* Element types. */
+enum { FAH_TYPE_F32 = 0, FAH_TYPE_F16 = 1, FAH_TYPE_BF16 = 2 };
+
+/* Causal attention over whole prompts, packed one behind the other, with
+ * grouped heads. Sequence s has the query rows query_offsets[s] to
+ * query_offsets[s + 1] and the key and value rows key_offsets[s] to
+ * key_offsets[s + 1]; its last query sees its last key, so with Lq queries and
+ * Lk keys query i sees the keys j <= i + Lk - Lq (Lk > Lq: the first Lk - Lq
+ * rows were cached before). Per query head h, with K/V head h / (heads /
+ * kv_heads): softmax(scale q k) over the keys seen, times their values, in
+ * 32-bit sums. A query that sees no key (Lk < Lq, or none at all), or whose
+ * every score is -infinity, gets zeros. Keys and values that a query does not
+ * see never reach its output, whatever they hold. Output rows of no sequence
+ * are left as they were. */
+typedef struct fah_packed_attention {
+    const void* query;  /* [query_rows][heads][head_size] */
+    const void* key;    /* [key_rows][kv_heads][head_size] */
+    const void* value;
+    void* output;       /* as query, of its type */
+    int64_t query_row, query_head, key_row, key_head, value_row, value_head, output_row, output_head; /* strides */
+    const int32_t* query_offsets; /* [sequences + 1], not falling; offsets outside 0..query_rows are taken as the nearer end */
+    const int32_t* key_offsets;   /* [sequences + 1], within 0..key_rows; NULL: query_offsets */
+    int sequences, query_rows, key_rows;
+    int longest_query, longest_key; /* most rows of one sequence: they only steer how the work is split */
+    int heads, kv_heads, head_size; /* heads a multiple of kv_heads */
+    int query_type, cache_type;     /* F32 with F16, F16 with F16, BF16 with BF16 */
+    float scale;                    /* above 0 */
+    void* workspace;
+    int64_t workspace_bytes;
+} fah_packed_attention;
+
+/* Declines head sizes that are no multiple of 8 or above 128, other pairs of
+ * types, and rows that do not start on 16 bytes (addresses and strides). */
+int fah_attention_packed_device(fah_context* context, const fah_packed_attention* call);
+int fah_attention_packed_workspace(const fah_packed_attention* call, int64_t* bytes);
+
+/* Attention of one token for each sequence of a batch whose sequences share
+ * their first `prefix` keys and values (one copy, read once for all; the
+ * device-side form of what CachePrefix and RestorePrefix keep per decoder,
+ * src/FunAsrNet/QwenDecoder.cs:122-137), followed by each sequence's own
+ * lengths[s] cache rows: softmax over both together, in 32-bit sums, heads
+ * grouped as in fah_packed_attention. prefix 0 is attention over the own rows
+ * alone. A token that sees no key, or whose every score is -infinity, gets
+ * zeros. Cache rows from lengths[s] on are not read. */
+typedef struct fah_prefix_attention {
+    const void* query;        /* [sequences][heads][head_size] */
+    const void* prefix_key;   /* [prefix][kv_heads][head_size] */
+    const void* prefix_value;
+    const void* key;          /* [sequences][capacity][kv_heads][head_size] */
+    const void* value;
+    void* output;             /* as query, of its type */
+    const int32_t* lengths;   /* [sequences]; below 0 counts as 0, above capacity as capacity */
+    int64_t query_sequence, query_head, prefix_key_row, prefix_key_head, prefix_value_row, prefix_value_head,
+        key_sequence, key_row, key_head, value_sequence, value_row, value_head, output_sequence, output_head; /* strides */
+    int sequences, prefix, capacity;
+    int longest;              /* most own rows of one sequence: it only steers how the work is split */
+    int heads, kv_heads, head_size;
+    int query_type, cache_type;
+    float scale;
+    void* workspace;
+    int64_t workspace_bytes;
+} fah_prefix_attention;
+
+/* Declines what fah_attention_packed_device declines. */
+int fah_attention_prefix_device(fah_context* context, const fah_prefix_attention* call);
+int fah_attention_prefix_workspace(const fah_prefix_attention* call, int64_t* bytes);
+
+/* Logits [rows][vocab] under penalties for repeated tokens, biases and
+ * grammar masks, and the greedy choice after them. Per row and token t, in
+ * fp32 and in this order:
+ *   a token of the row's history:         x > 0 ? x / repetition : x * repetition
+ *   n times in it behind the prompt:      x - frequency * n, then x - presence
+ *   in the bias list (the last entry):    x + bias
+ *   bit t % 32 of the mask's word t / 32 clear:  -infinity
+ * then rounded to the type and written to output. tokens[r] is the largest
+ * written value's token, the lowest of equal ones (QwenDecoder.Greedy's order,
+ * src/FunAsrNet/QwenDecoder.cs:278-326); NaN and -infinity are never chosen,
+ * and -1 says that nothing is left. List entries outside 0..vocab - 1 are
+ * passed over, so -1 may fill a list up. */
+typedef struct fah_logits_adjust {
+    const void* logits;
+    void* output;    /* may be logits, with the same stride */
+    int32_t* tokens; /* [rows]; NULL: not asked for */
+    int64_t logits_stride, output_stride; /* between rows */
+    int rows, vocab, type;
+    int history_capacity;          /* entries of a history row; 0: none */
+    const int32_t* history;        /* rows history_stride apart; 0: one for all rows */
+    int64_t history_stride;
+    const int32_t* history_counts; /* [rows] entries in use, at most the capacity; NULL: all */
+    const int32_t* prompt_counts;  /* [rows] the first ones, which are the prompt; NULL: 0 */
+    const float* repetition;       /* [rows]; NULL: 1 */
+    const float* presence;         /* [rows]; NULL: 0 */
+    const float* frequency;        /* [rows]; NULL: 0 */
+    const int32_t* bias_tokens;    /* rows bias_stride apart; 0: one for all rows */
+    const float* bias_values;      /* laid out alike */
+    int64_t bias_stride;
+    int bias_capacity;             /* entries of a bias row; 0: none */
+    int mask_rows;                 /* 0: none */
+    const int32_t* bias_counts;    /* [rows]; NULL: all */
+    const uint32_t* masks;         /* [mask_rows][(vocab + 31) / 32] words, rows mask_stride apart */
+    int64_t mask_stride;
+    const int32_t* mask_index;     /* [rows] the mask row of each row, outside 0..mask_rows - 1: no mask;
+                                    * NULL: row r has mask r, or all have mask 0 if mask_rows is 1 */
+    void* workspace;
+    int64_t workspace_bytes;
+} fah_logits_adjust;
+
+/* Declines other types. */
+int fah_logits_adjust_device(fah_context* context, const fah_logits_adjust* call);
+int fah_logits_adjust_workspace(const fah_logits_adjust* call, int64_t* bytes);
+
 /* Decoder ------------------------------------------------------------------- */
 
 typedef struct fah_decoder_config {

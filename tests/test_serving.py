@@ -1,0 +1,93 @@
+"""Refusals and sizes of the serving operators that need no device: the
+*_workspace calls check a descriptor as the device calls do."""
+import ctypes
+
+import pytest
+
+from funasrnet_amd import hip
+
+
+def packed(**changes):
+    a = hip.PackedAttention(query_row=2048, query_head=128, key_row=1024, key_head=128, value_row=1024, value_head=128,
+                            output_row=2048, output_head=128, sequences=3, query_rows=100, key_rows=120, longest_query=50,
+                            longest_key=60, heads=16, kv_heads=8, head_size=128, query_type=hip.TYPE_F32,
+                            cache_type=hip.TYPE_F16, scale=0.1)
+    for name, value in changes.items():
+        setattr(a, name, value)
+    return a
+
+
+def prefix(**changes):
+    a = hip.PrefixAttention(query_sequence=2048, query_head=128, prefix_key_row=128, prefix_key_head=128 * 500,
+                            prefix_value_row=128, prefix_value_head=128 * 500, key_sequence=1 << 20, key_row=128,
+                            key_head=1 << 17, value_sequence=1 << 20, value_row=128, value_head=1 << 17,
+                            output_sequence=2048, output_head=128, sequences=5, prefix=500, capacity=1024, longest=700,
+                            heads=16, kv_heads=8, head_size=128, query_type=hip.TYPE_F32, cache_type=hip.TYPE_F16, scale=0.1)
+    for name, value in changes.items():
+        setattr(a, name, value)
+    return a
+
+
+def logits(**changes):
+    a = hip.LogitsAdjust(logits_stride=1000, output_stride=1000, rows=4, vocab=1000, type=hip.TYPE_F32, tokens=16)
+    for name, value in changes.items():
+        setattr(a, name, value)
+    return a
+
+
+CALLS = {"packed": ("fah_attention_packed", packed), "prefix": ("fah_attention_prefix", prefix),
+         "logits": ("fah_logits_adjust", logits)}
+
+
+def workspace(kind, **changes):
+    name, make = CALLS[kind]
+    v = ctypes.c_int64(-7)
+    rc = getattr(hip.load(), name + "_workspace")(ctypes.byref(make(**changes)), ctypes.byref(v))
+    return rc, v.value
+
+
+@pytest.mark.parametrize("kind", CALLS)
+def test_workspace_is_given(kind):
+    rc, n = workspace(kind)
+    assert rc == hip.OK and n >= 0
+
+
+@pytest.mark.parametrize("kind", CALLS)
+def test_null_arguments(kind):
+    lib, (name, make) = hip.load(), CALLS[kind]
+    v = ctypes.c_int64()
+    assert getattr(lib, name + "_workspace")(None, ctypes.byref(v)) == hip.ERROR_ARGUMENT
+    assert getattr(lib, name + "_workspace")(ctypes.byref(make()), None) == hip.ERROR_ARGUMENT
+    assert getattr(lib, name + "_device")(None, ctypes.byref(make())) == hip.ERROR_ARGUMENT
+
+
+@pytest.mark.parametrize("kind,changes", [
+    ("packed", dict(sequences=-1)), ("packed", dict(query_rows=-1)), ("packed", dict(key_rows=-1)),
+    ("packed", dict(longest_query=-1)), ("packed", dict(longest_key=-1)), ("packed", dict(heads=0)),
+    ("packed", dict(kv_heads=0)), ("packed", dict(kv_heads=3)), ("packed", dict(head_size=0)), ("packed", dict(scale=0.0)),
+    ("packed", dict(scale=-1.0)), ("packed", dict(scale=float("nan"))), ("packed", dict(scale=float("inf"))),
+    ("packed", dict(query_rows=2**31 - 1)), ("packed", dict(sequences=2**31 - 1)),
+    ("prefix", dict(sequences=-1)), ("prefix", dict(prefix=-1)), ("prefix", dict(capacity=-1)), ("prefix", dict(longest=-1)),
+    ("prefix", dict(heads=15)), ("prefix", dict(kv_heads=-8)), ("prefix", dict(scale=0.0)),
+    ("prefix", dict(sequences=2**31 - 1)),
+    ("logits", dict(rows=-1)), ("logits", dict(vocab=-1)), ("logits", dict(rows=70000)), ("logits", dict(history_capacity=-1)),
+    ("logits", dict(bias_capacity=-1)), ("logits", dict(mask_rows=-1)), ("logits", dict(vocab=2**31 - 1)),
+])
+def test_invalid_sizes_are_errors(kind, changes):
+    rc, n = workspace(kind, **changes)
+    assert rc == hip.ERROR_ARGUMENT and n == -7
+    assert hip.load().fah_last_error()
+
+
+@pytest.mark.parametrize("kind,changes", [
+    ("packed", dict(head_size=12)), ("packed", dict(head_size=136)), ("packed", dict(query_type=hip.TYPE_F32, cache_type=0)),
+    ("packed", dict(query_type=hip.TYPE_F16, cache_type=hip.TYPE_BF16)), ("packed", dict(query_type=7)),
+    ("packed", dict(query_row=2046)), ("packed", dict(output_head=130)), ("packed", dict(key_row=1028)),
+    ("packed", dict(value_head=-128)),
+    ("prefix", dict(head_size=100)), ("prefix", dict(cache_type=hip.TYPE_BF16)), ("prefix", dict(prefix_key_row=132)),
+    ("prefix", dict(key_sequence=(1 << 20) + 4)), ("prefix", dict(query_head=2)), ("prefix", dict(output_sequence=-2048)),
+    ("logits", dict(type=3)), ("logits", dict(type=-1)),
+])
+def test_unsupported_forms_are_declined(kind, changes):
+    rc, n = workspace(kind, **changes)
+    assert rc == hip.DECLINED and n == -7
