@@ -2136,6 +2136,10 @@ void require_workspace(const void* p, int64_t have, int64_t need) {
           "the workspace needs " + std::to_string(need) + " bytes at a 16-byte boundary");
 }
 
+// Most elements between two key or value rows: the kernels' offsets within 16
+// rows are 32-bit byte offsets.
+constexpr int64_t kRowStride = 1 << 26;
+
 // False: declined.
 bool check_packed(const fah_packed_attention& a) {
   require(a.sequences >= 0 && a.query_rows >= 0 && a.key_rows >= 0 && a.longest_query >= 0 && a.longest_key >= 0,
@@ -2147,7 +2151,8 @@ bool check_packed(const fah_packed_attention& a) {
           "too many query rows or sequences");
   return fah::attention_supported(a.heads, a.kv_heads, a.head_size, a.query_type, a.cache_type) &&
          strides16(a.query_type, {a.query_row, a.query_head, a.output_row, a.output_head}) &&
-         strides16(a.cache_type, {a.key_row, a.key_head, a.value_row, a.value_head});
+         strides16(a.cache_type, {a.key_row, a.key_head, a.value_row, a.value_head}) &&
+         a.key_row <= kRowStride && a.value_row <= kRowStride;
 }
 
 bool check_prefix(const fah_prefix_attention& a) {
@@ -2159,7 +2164,8 @@ bool check_prefix(const fah_prefix_attention& a) {
   return fah::attention_supported(a.heads, a.kv_heads, a.head_size, a.query_type, a.cache_type) &&
          strides16(a.query_type, {a.query_sequence, a.query_head, a.output_sequence, a.output_head}) &&
          strides16(a.cache_type, {a.prefix_key_row, a.prefix_key_head, a.prefix_value_row, a.prefix_value_head,
-                                  a.key_sequence, a.key_row, a.key_head, a.value_sequence, a.value_row, a.value_head});
+                                  a.key_sequence, a.key_row, a.key_head, a.value_sequence, a.value_row, a.value_head}) &&
+         std::max({a.prefix_key_row, a.prefix_value_row, a.key_row, a.value_row}) <= kRowStride;
 }
 
 bool check_logits(const fah_logits_adjust& a) {

@@ -4,114 +4,806 @@
 #include "fah_device.h"
 #include "fah_internal.h"
 
-#include <hip/hip_bf16.h>
+#include <algorithm>
+#include <type_traits>
 
 namespace fah {
 namespace {
 
-template <typename T>
-__device__ __forceinline__ float widen(T v) {
-  return (float)v;
-}
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using s16x4 = __attribute__((ext_vector_type(4))) short;
+using s16x8 = __attribute__((ext_vector_type(8))) short;
+using LdsTr = s16x4 __attribute__((address_space(3))) *;
+using LdsFrag = s16x8 __attribute__((address_space(3))) *;
+using LdsDma = __attribute__((address_space(3))) void*;
+
+constexpr int kThreads = 256;
+constexpr float kInf = __builtin_inff();
+constexpr float kLog2e = 1.44269504088896340736f;
+// Weights are held as 2^(score - reference + kLift): at most 2^(kLift + kSlack)
+// = 2^14, which fp16 holds, so that small weights keep fp16's full precision
+// down to 2^-22 of the largest one. The reference only moves when a row's
+// largest score has risen by more than kSlack.
+constexpr float kLift = 8.0f, kSlack = 6.0f;
 
 __device__ __forceinline__ int clamp_int(int v, int low, int high) { return v < low ? low : v > high ? high : v; }
 
-// Running softmax of one query row over keys, a wave per row: lane l holds the
-// channels l and l + 64.
+// a * b + c of 32 x 32 x 16 blocks, 16-bit operands of type T.
+template <typename T>
+__device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
+  if constexpr (std::is_same_v<T, __bf16>)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// The value of lane l ^ 32.
+__device__ __forceinline__ float other_half(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
+  return u2f(threadIdx.x & 32 ? r[0] : r[1]);
+}
+
+// What one workgroup attends: BM rows (of one K/V head: the row r is token r /
+// group, query head r % group of the head's group) over the keys [begin, end).
 template <typename Q, typename K>
-struct Row {
-  float q[2], o[2], top = -__builtin_inff(), total = 0.0f;
-  int size, lane;
-  __device__ Row(const Q* query, int n) : size(n), lane(threadIdx.x) {
-    for (int i = 0; i < 2; ++i) {
-      q[i] = lane + 64 * i < n ? widen(query[lane + 64 * i]) : 0.0f;
-      o[i] = 0.0f;
+struct Task {
+  const Q* q;                // token 0, the K/V head's first query head
+  int64_t q_token, q_head;   // strides
+  const K *k, *v;            // key 0
+  unsigned k_row, v_row;     // strides
+  int row0, rows, group;     // rows row0 .. row0 + rows - 1
+  int begin, end;            // keys
+  int first_limit;           // token 0 sees the keys below this; per token one more if causal
+  bool causal;
+  __device__ int limit(int row) const {
+    const int64_t n = (int64_t)first_limit + (causal ? row / group : 0);
+    return n < end ? (int)n : end;
+  }
+  __device__ const Q* query(int row) const { return q + (row / group) * q_token + (row % group) * q_head; }
+};
+
+// Where it goes: the finished rows, or partial sums for combine_*: per row
+// [size] sums, then the reference and the total.
+template <typename Q>
+struct Sink {
+  Q* out;                    // token 0, the K/V head's first query head; null: partial
+  int64_t o_token, o_head;
+  float* sums;               // of row row0: [rows][D]
+  float* marks;              // [rows][2]
+};
+
+template <int D>
+struct Tile {
+  static constexpr int kChunks = D / 8;               // 16-byte chunks a row
+  static constexpr int kRowsLoad = 64 / kChunks;      // rows a wave loads at a time
+  static constexpr int kRowBytes = 2 * D;
+  // Chunk c of row r sits at place c ^ swizzle(r): fragment reads (16 rows, one
+  // chunk) of keys and transposing reads (4 rows, 64 bytes) of values then
+  // touch all 64 banks.
+  __device__ static int key_swizzle(int r) { return D == 128 ? r & 15 : (r >> 1) & 7; }
+  __device__ static int value_swizzle(int r) { return D == 128 ? (r & 3) << 2 : (r & 2) << 1; }
+};
+
+// 16 bytes a lane from base + offset to LDS at `to` + 16 lane. Inline, because
+// the compiler would wait for a load into LDS before any read of LDS: the
+// tiles' reads are ordered by wait_loads and a barrier instead. (It has no
+// register that it writes; a load into M0's place needs one wait state.)
+__device__ __forceinline__ void load_lds(const void* base, unsigned offset, unsigned to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_lds(const void* from, unsigned to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+}
+// Every load of this wave is done (vmcnt 0, nothing else waited for). A barrier
+// follows: reads of LDS may move up to it but not before it.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+
+// Loads tiles of ROWS keys or values by the waves w of W, kRowsLoad rows a load.
+// A lane's place in the source repeats, but for the base, after the rows whose
+// swizzles differ: its offsets are kept, and the base moves in scalar registers.
+template <typename K, int D, int ROWS, int W, bool VALUES>
+struct Loader {
+  using T = Tile<D>;
+  static constexpr int kLoads = ROWS / T::kRowsLoad / W, kStep = W * T::kRowsLoad;
+  static constexpr int kPeriod = VALUES ? 4 : 16;      // rows after which the swizzle repeats
+  static constexpr int kKinds = kStep >= kPeriod ? 1 : kPeriod / kStep;
+  static_assert(kLoads >= 1 && kLoads % kKinds == 0);
+  unsigned offset[kKinds];
+  unsigned to;       // LDS place of the wave's first load
+  int row0;          // its first row in the tile
+
+  __device__ static int chunk(int r) {
+    return (int)(threadIdx.x & 63) % T::kChunks ^ (VALUES ? T::value_swizzle(r) : T::key_swizzle(r));
+  }
+  __device__ Loader(const unsigned char* tile, unsigned stride, int w)
+      : to(lds_address(tile) + w * 1024), row0(w * T::kRowsLoad) {
+#pragma unroll
+    for (int j = 0; j < kKinds; ++j) {
+      const int r = row0 + j * kStep + (threadIdx.x & 63) / T::kChunks;
+      offset[j] = (unsigned)r * stride * 2 + chunk(r) * 16;
     }
   }
-  __device__ void add(const K* k, const K* v, int64_t k_row, int64_t v_row, int count, float scale) {
-    for (int t = 0; t < count; ++t) {
-      float s = 0.0f;
-      for (int i = 0; i < 2; ++i)
-        if (lane + 64 * i < size) s += q[i] * widen(k[t * k_row + lane + 64 * i]);
-      for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
-      s *= scale;
-      const float next = s > top || s != s ? s : top;
-      const float base = next == -__builtin_inff() ? 0.0f : next;
-      const float keep = expf(top - base), p = expf(s - base);
-      total = total * keep + p;
-      for (int i = 0; i < 2; ++i)
-        if (lane + 64 * i < size) o[i] = o[i] * keep + p * widen(v[t * v_row + lane + 64 * i]);
-      top = next;
+  // Rows first ..: `shift` is the place of this buffer behind the constructor's.
+  __device__ __forceinline__ void load(const K* base, unsigned stride, int first, int last, unsigned shift, int size) const {
+    const bool whole = first + ROWS - 1 <= last && size == D;
+    if (whole) {
+      const K* at = base + (int64_t)first * stride;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        load_lds(at + (int64_t)(i / kKinds * kKinds * kStep) * stride, offset[i % kKinds], to + shift + i * W * 1024);
+    } else {
+      // Rows past `last` repeat it (their scores are masked); places behind
+      // head_size stay as they are (zero).
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int r = row0 + i * kStep + (threadIdx.x & 63) / T::kChunks;
+        const int row = first + r < last ? first + r : last;
+        if (chunk(r) * 8 < size) load_lds(base + (int64_t)row * stride + chunk(r) * 8, to + shift + i * W * 1024);
+      }
     }
-  }
-  __device__ void write(Q* out) const {
-    for (int i = 0; i < 2; ++i)
-      if (lane + 64 * i < size) out[lane + 64 * i] = (Q)(total == 0.0f ? 0.0f : o[i] / total);
   }
 };
 
+// A row by one wave, channels 2 lane and 2 lane + 1, only keys that it sees
+// read: for rows whose tile held infinities or NaN where they are masked.
+// The lane's two sums, then the row's reference and total.
 template <typename Q, typename K>
-__global__ __launch_bounds__(64) void packed_rows_kernel(fah_packed_attention a) {
-  const int row = blockIdx.x, head = blockIdx.y, kv = head / (a.heads / a.kv_heads);
-  int lo = -1, begin = 0, end = 0;
-  for (int s = 0; s < a.sequences; ++s) {
-    begin = clamp_int(a.query_offsets[s], 0, a.query_rows);
-    end = clamp_int(a.query_offsets[s + 1], 0, a.query_rows);
-    if (row >= begin && row < end) {
-      lo = s;
-      break;
-    }
+__device__ __noinline__ f32x4 slow_row(const Q* q, const K* k, const K* v_rows, unsigned k_row, unsigned v_row, int begin,
+                                       int lim, int size, float scale) {
+  const int lane = threadIdx.x & 63;
+  float x[2] = {}, sum[2] = {}, top = -kInf, total = 0.0f;
+  for (int i = 0; i < 2; ++i)
+    if (2 * lane + i < size) x[i] = (float)q[2 * lane + i];
+  for (int key = begin; key < lim; ++key) {
+    float s = 0.0f, v[2] = {};
+    for (int i = 0; i < 2; ++i)
+      if (2 * lane + i < size) {
+        s += x[i] * (float)k[(int64_t)key * k_row + 2 * lane + i];
+        v[i] = (float)v_rows[(int64_t)key * v_row + 2 * lane + i];
+      }
+    for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
+    s *= scale * kLog2e;
+    const float next = s > top || s != s ? s : top;
+    const float base = next == -kInf ? 0.0f : next;
+    const float keep = __builtin_amdgcn_exp2f(top - base), p = __builtin_amdgcn_exp2f(s - base);
+    total = total * keep + p;
+    for (int i = 0; i < 2; ++i) sum[i] = sum[i] * keep + p * v[i];
+    top = next;
   }
-  if (lo < 0) return;
-  const int* offsets = a.key_offsets ? a.key_offsets : a.query_offsets;
-  const int kb = clamp_int(offsets[lo], 0, a.key_rows), ke = clamp_int(offsets[lo + 1], kb, a.key_rows);
-  int count = (row - begin) + (ke - kb) - (end - begin) + 1;
-  count = clamp_int(count, 0, ke - kb);
-  Row<Q, K> r(static_cast<const Q*>(a.query) + row * a.query_row + head * a.query_head, a.head_size);
-  r.add(static_cast<const K*>(a.key) + kb * a.key_row + kv * a.key_head,
-        static_cast<const K*>(a.value) + kb * a.value_row + kv * a.value_head, a.key_row, a.value_row, count, a.scale);
-  r.write(static_cast<Q*>(a.output) + row * a.output_row + head * a.output_head);
+  return f32x4{sum[0], sum[1], top, total};
 }
 
-template <typename Q, typename K>
-__global__ __launch_bounds__(64) void prefix_rows_kernel(fah_prefix_attention a) {
-  const int s = blockIdx.x, head = blockIdx.y, kv = head / (a.heads / a.kv_heads);
-  Row<Q, K> r(static_cast<const Q*>(a.query) + s * a.query_sequence + head * a.query_head, a.head_size);
-  r.add(static_cast<const K*>(a.prefix_key) + kv * a.prefix_key_head,
-        static_cast<const K*>(a.prefix_value) + kv * a.prefix_value_head, a.prefix_key_row, a.prefix_value_row, a.prefix,
-        a.scale);
-  r.add(static_cast<const K*>(a.key) + s * a.key_sequence + kv * a.key_head,
-        static_cast<const K*>(a.value) + s * a.value_sequence + kv * a.value_head, a.key_row, a.value_row,
-        clamp_int(a.lengths[s], 0, a.capacity), a.scale);
-  r.write(static_cast<Q*>(a.output) + s * a.output_sequence + head * a.output_head);
+// A 16-bit type's packed pair.
+template <typename K>
+__device__ __forceinline__ unsigned pack2(float a, float b) {
+  if constexpr (std::is_same_v<K, __bf16>) {
+    using V = __attribute__((ext_vector_type(2))) __bf16;
+    return __builtin_bit_cast(unsigned, V{(__bf16)a, (__bf16)b});
+  } else {
+    using V = __attribute__((ext_vector_type(2))) _Float16;
+    return __builtin_bit_cast(unsigned, V{(_Float16)a, (_Float16)b});
+  }
+}
+
+// The workgroup's four waves as WR groups of 32 rows times WK shares of each
+// key tile; a wave takes NK keys of a tile.
+template <typename Q, typename K, int D, int WR, int WK, int NK>
+struct Core {
+  static constexpr int BM = 32 * WR, TR = WK * NK;
+  static constexpr int kTileBytes = TR * 2 * D;        // keys, or values
+  static constexpr bool kSplit = std::is_same_v<Q, float>;
+  static constexpr int kSteps = D / 16;
+
+  // lds: two buffers of a key tile and a value tile; at the end the waves'
+  // sums. marks: [4][32][2].
+  __device__ static void run(const Task<Q, K>& t, const Sink<Q>& sink, int size, float scale, unsigned char* lds,
+                             float* marks) {
+    static_assert(kTileBytes >= 32 * D * 4);
+    using T = Tile<D>;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
+    const int wr = wave / WK, wk = wave % WK;
+    const int my_row = wr * 32 + col;
+    const bool valid = my_row < t.rows;
+    const int lim = valid ? t.limit(t.row0 + my_row) : 0;
+    const int wave_rows = clamp_int(t.rows - wr * 32, 0, 32);
+    const int lim_low = wave_rows ? t.limit(t.row0 + wr * 32) : 0;
+    const int lim_high = wave_rows ? t.limit(t.row0 + wr * 32 + wave_rows - 1) : 0;
+    const int end = t.rows ? t.limit(t.row0 + t.rows - 1) : 0;  // of the workgroup
+    const int last = t.end - 1;
+
+    if (D != size) {
+      for (int i = tid; i < 4 * kTileBytes / 16; i += kThreads) reinterpret_cast<uint4*>(lds)[i] = uint4{0, 0, 0, 0};
+      __syncthreads();
+    }
+    // With one group of rows a wave loads the keys that it takes itself.
+    constexpr int kOwn = WR == 1 ? NK : TR, kLoaders = WR == 1 ? 1 : 4;
+    const int own = WR == 1 ? wave * NK : 0, loader = WR == 1 ? 0 : wave;
+    const Loader<K, D, kOwn, kLoaders, false> keys(lds + own * T::kRowBytes, t.k_row, loader);
+    const Loader<K, D, kOwn, kLoaders, true> values(lds + kTileBytes + own * T::kRowBytes, t.v_row, loader);
+    auto load = [&](int buffer, int key) {
+      keys.load(t.k, t.k_row, key + own, last, buffer * 2 * kTileBytes, size);
+      values.load(t.v, t.v_row, key + own, last, buffer * 2 * kTileBytes, size);
+    };
+    if (t.begin < end) load(0, t.begin);
+
+    // Queries: the B operand, lane (row col, channels 16 s + 8 half ..). fp32
+    // queries are scaled by a power of two to below 2^14 and split into two
+    // fp16 parts (22 bits; the scale keeps the second part normal).
+    s16x8 qf[kSplit ? 2 : 1][kSteps];
+    float c = scale * kLog2e;
+    {
+      const Q* q = t.query(t.row0 + (valid ? my_row : 0));
+      if constexpr (kSplit) {
+        f32x4 x[kSteps][2];
+        float most = 0.0f;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int d = 16 * s + 8 * half + 4 * i;
+            x[s][i] = valid && d < size ? *reinterpret_cast<const f32x4*>(q + d) : f32x4{};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(x[s][i][j]));
+          }
+        most = fmaxf(most, other_half(most));
+        const int e = (int)(f2u(most) >> 23) - 127;
+        const int up = e == 128 ? 0 : clamp_int(13 - e, -114, 126);
+        const float lift = u2f((unsigned)(up + 127) << 23);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          f16x8 hi, lo;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float v = x[s][j >> 2][j & 3] * lift;
+            hi[j] = (_Float16)v;
+            lo[j] = (_Float16)(v - (float)hi[j]);
+          }
+          qf[0][s] = __builtin_bit_cast(s16x8, hi);
+          qf[kSplit ? 1 : 0][s] = __builtin_bit_cast(s16x8, lo);
+        }
+        c = fmaxf(c * u2f((unsigned)(127 - up) << 23), 1.2e-38f);
+      } else {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          const int d = 16 * s + 8 * half;
+          qf[0][s] = valid && d < size ? *reinterpret_cast<const s16x8*>(q + d) : s16x8{};
+        }
+      }
+    }
+
+    f32x16 acc[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] = f32x16{};
+    float ref = -kInf, total = 0.0f;
+    bool masked = false;
+
+    // Fragment places within a tile. Keys: lane's row, chunk 2 s + half.
+    // Values: lane 16 g + i of a half reads row i / 4 of four, 8 bytes of the
+    // 32 that are channels 16 g .. 16 g + 15, and gets channel i of the four rows.
+    const int key_at = (wk * NK + col) * T::kRowBytes, key_sw = T::key_swizzle(col);
+    const int vi = lane & 15, vg = (lane >> 4) & 1;
+    const int value_at = (wk * NK + 4 * half + vi / 4) * T::kRowBytes + (vi & 1) * 8;
+    const int value_sw = T::value_swizzle(vi / 4), value_chunk = 2 * vg + ((vi & 3) >> 1);
+
+    auto compute = [&](int buffer, int key0) {
+      const unsigned char* kt = lds + buffer * 2 * kTileBytes;
+      const unsigned char* vt = kt + kTileBytes;
+      f32x16 s[NK / 32];
+#pragma unroll
+      for (int b = 0; b < NK / 32; ++b) s[b] = f32x16{};
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step)
+#pragma unroll
+        for (int b = 0; b < NK / 32; ++b) {
+          const s16x8 kf = *(LdsFrag)(kt + key_at + b * 32 * T::kRowBytes + (((2 * step + half) ^ key_sw) << 4));
+          s[b] = mfma<K>(kf, qf[0][step], s[b]);
+          if constexpr (kSplit) s[b] = mfma<K>(kf, qf[kSplit ? 1 : 0][step], s[b]);
+        }
+      if (key0 + NK > lim_low) {
+        masked = true;
+        const int room = lim - key0 - 4 * half;
+#pragma unroll
+        for (int b = 0; b < NK / 32; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[b][i] = 32 * b + 8 * (i >> 2) + (i & 3) < room ? s[b][i] : -kInf;
+      }
+      float top = -kInf;
+#pragma unroll
+      for (int b = 0; b < NK / 32; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+      top = fmaxf(top, other_half(top)) * c;
+      const bool rise = top > ref + kSlack;
+      if (__builtin_amdgcn_ballot_w64(rise) != 0) {
+        const float keep = rise ? __builtin_amdgcn_exp2f(ref - top) : 1.0f;
+        ref = rise ? top : ref;
+        total *= keep;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) acc[i] *= keep;
+      }
+      const float base = ref == -kInf ? 0.0f : kLift - ref;
+#pragma unroll
+      for (int b = 0; b < NK / 32; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, base));
+          total += s[b][i];
+        }
+#pragma unroll
+      for (int step = 0; step < NK / 16; ++step) {
+        // The B operand of 16 keys: a lane's eight weights as they are; the
+        // values are read in the same key order.
+        uint4 hi, lo;
+        unsigned* ph = reinterpret_cast<unsigned*>(&hi);
+        unsigned* pl = reinterpret_cast<unsigned*>(&lo);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float a = s[step >> 1][8 * (step & 1) + 2 * i], b = s[step >> 1][8 * (step & 1) + 2 * i + 1];
+          ph[i] = pack2<K>(a, b);
+          if constexpr (kSplit) {
+            using V = __attribute__((ext_vector_type(2))) _Float16;
+            const V h = __builtin_bit_cast(V, ph[i]);
+            pl[i] = pack2<K>(a - (float)h[0], b - (float)h[1]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const unsigned char* at = vt + value_at + step * 16 * T::kRowBytes + (((4 * i + value_chunk) ^ value_sw) << 4);
+          const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr)(at));
+          const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr)(at + 8 * T::kRowBytes));
+          const s16x8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+          acc[i] = mfma<K>(vf, __builtin_bit_cast(s16x8, hi), acc[i]);
+          if constexpr (kSplit) acc[i] = mfma<K>(vf, __builtin_bit_cast(s16x8, lo), acc[i]);
+        }
+      }
+    };
+
+    // One pass a buffer. The barrier: this buffer's tile is here, and the other
+    // one's readers are done.
+    auto pass = [&](int buffer, int key) {
+      wait_loads();
+      __syncthreads();
+      if (key + TR < end) load(buffer ^ 1, key + TR);
+      if (key + wk * NK < lim_high) compute(buffer, key + wk * NK);
+    };
+    for (int key = t.begin; key < end; key += 2 * TR) {
+      pass(0, key);
+      if (key + TR < end) pass(1, key + TR);
+    }
+    total += other_half(total);
+
+    // Sums, [wave][32 rows][D] with the 16-byte chunks of a row swizzled; then
+    // every row by half a wave.
+    __syncthreads();
+    float* sums = reinterpret_cast<float*>(lds) + wave * 32 * D;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int chunk = 8 * i + 2 * j + half;
+        *reinterpret_cast<f32x4*>(sums + col * D + ((chunk ^ (col & (D / 4 - 1))) << 2)) =
+            f32x4{acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]};
+      }
+    if (half == 0) {
+      marks[(wave * 32 + col) * 2] = ref - kLift;
+      marks[(wave * 32 + col) * 2 + 1] = total;
+    }
+    const bool any_masked = __syncthreads_or(masked);
+    constexpr int kLanes = D / 4;  // lanes a row, four channels each
+    for (int r0 = wave * (64 / kLanes); r0 < t.rows; r0 += 4 * (64 / kLanes)) {
+      const int r = r0 + lane / kLanes, chunk = lane % kLanes;
+      float o[4] = {}, top = -kInf, sum = 0.0f;
+      if (r < t.rows) {
+        const int w0 = (r / 32) * WK, rc = r % 32;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) top = fmaxf(top, marks[((w0 + w) * 32 + rc) * 2]);
+#pragma unroll
+        for (int w = 0; w < WK; ++w) {
+          const float m = marks[((w0 + w) * 32 + rc) * 2];
+          const float keep = m == -kInf ? 0.0f : m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+          sum += keep * marks[((w0 + w) * 32 + rc) * 2 + 1];
+          const f32x4 v = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds) + ((w0 + w) * 32 + rc) * D + ((chunk ^ (rc & (D / 4 - 1))) << 2));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] += m == -kInf && v[i] == v[i] ? 0.0f : keep * v[i];
+        }
+      }
+      if (any_masked) {
+        const bool bad = r < t.rows && 4 * chunk < size && !(fabsf(o[0]) + fabsf(o[1]) + fabsf(o[2]) + fabsf(o[3]) < kInf);
+        unsigned long long rows_bad = __builtin_amdgcn_ballot_w64(bad);
+        for (int g = 0; g < 64 / kLanes; ++g) {
+          if (!(rows_bad >> (g * kLanes) & (kLanes == 64 ? ~0ull : (1ull << kLanes) - 1))) continue;
+          const int row = t.row0 + r0 + g;
+          const f32x4 v = slow_row(t.query(row), t.k, t.v, t.k_row, t.v_row, t.begin, t.limit(row), size, scale);
+          // Lane l holds channels 2 l, 2 l + 1.
+          float w[4];
+          for (int i = 0; i < 4; ++i) w[i] = __shfl(i & 1 ? v[1] : v[0], 2 * chunk + (i >> 1), 64);
+          if (lane / kLanes == g) {
+            for (int i = 0; i < 4; ++i) o[i] = w[i];
+            top = v[2];
+            sum = v[3];
+          }
+        }
+      }
+      if (r < t.rows && 4 * chunk < size) {
+        const int row = t.row0 + r;
+        if (sink.out) {
+          const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+          Q* dst = sink.out + (row / t.group) * sink.o_token + (row % t.group) * sink.o_head + 4 * chunk;
+          if constexpr (kSplit) {
+            *reinterpret_cast<f32x4*>(dst) = f32x4{o[0] * inverse, o[1] * inverse, o[2] * inverse, o[3] * inverse};
+          } else {
+            *reinterpret_cast<uint2*>(dst) = uint2{pack2<K>(o[0] * inverse, o[1] * inverse), pack2<K>(o[2] * inverse, o[3] * inverse)};
+          }
+        } else {
+          *reinterpret_cast<f32x4*>(sink.sums + (size_t)r * D + 4 * chunk) = f32x4{o[0], o[1], o[2], o[3]};
+          if (chunk == 0) {
+            sink.marks[2 * r] = top;
+            sink.marks[2 * r + 1] = sum;
+          }
+        }
+      }
+    }
+  }
+};
+
+// ---- Packed prompts ---------------------------------------------------------------
+
+// The place of sequence s's first tile of BM rows among all tiles: sequences
+// may leave one tile each empty, so no sum over the earlier ones is needed.
+__device__ __forceinline__ int first_tile(const fah_packed_attention& a, int s, int group, int BM) {
+  return clamp_int(a.query_offsets[s], 0, a.query_rows) * group / BM + s;
+}
+
+// The sequence whose tile `slot` is, or -1: 64 probes at a time.
+__device__ __forceinline__ int find_sequence(const fah_packed_attention& a, int slot, int group, int BM) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, hi = a.sequences;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) / 64, probe = lo + lane * step;
+    const bool ok = probe < hi && first_tile(a, probe, group, BM) <= slot;
+    const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(ok));
+    if (n == 0) return -1;
+    lo += (n - 1) * step;
+    hi = lo + step < hi ? lo + step : hi;
+  }
+  return first_tile(a, lo, group, BM) <= slot ? lo : -1;
+}
+
+struct PackedTile {
+  int sequence, begin, row0, rows, key_begin, keys, first_limit;  // rows 0: none
+};
+
+__device__ __forceinline__ PackedTile packed_tile(const fah_packed_attention& a, int slot, int group, int BM) {
+  PackedTile p{};
+  p.sequence = __builtin_amdgcn_readfirstlane(find_sequence(a, slot, group, BM));
+  if (p.sequence < 0) return p;
+  const int* ko = a.key_offsets ? a.key_offsets : a.query_offsets;
+  p.begin = clamp_int(a.query_offsets[p.sequence], 0, a.query_rows);
+  const int queries = clamp_int(a.query_offsets[p.sequence + 1], p.begin, a.query_rows) - p.begin;
+  p.key_begin = clamp_int(ko[p.sequence], 0, a.key_rows);
+  p.keys = clamp_int(ko[p.sequence + 1], p.key_begin, a.key_rows) - p.key_begin;
+  p.first_limit = p.keys - queries + 1;
+  p.row0 = (slot - first_tile(a, p.sequence, group, BM)) * BM;
+  p.rows = clamp_int(queries * group - p.row0, 0, BM);
+  return p;
+}
+
+// Workgroup: (tile from the last one on, share of the keys, K/V head), the K/V
+// head fastest, so that with 8 of them each XCD's L2 serves one head.
+template <typename Q, typename K, int D, int WR, int WK, int NK>
+__global__ __launch_bounds__(kThreads) void packed_kernel(fah_packed_attention a, int slots, int splits) {
+  using C = Core<Q, K, D, WR, WK, NK>;
+  __shared__ __align__(16) unsigned char lds[4 * C::kTileBytes];
+  __shared__ float marks[256];
+  const int group = a.heads / a.kv_heads, head = blockIdx.x % a.kv_heads;
+  const int rest = blockIdx.x / a.kv_heads, split = rest % splits, slot = slots - 1 - rest / splits;
+  const PackedTile p = packed_tile(a, slot, group, C::BM);
+  if (p.rows == 0) return;
+  Task<Q, K> t;
+  t.q = static_cast<const Q*>(a.query) + p.begin * a.query_row + (int64_t)head * group * a.query_head;
+  t.q_token = a.query_row;
+  t.q_head = a.query_head;
+  t.k = static_cast<const K*>(a.key) + p.key_begin * a.key_row + head * a.key_head;
+  t.v = static_cast<const K*>(a.value) + p.key_begin * a.value_row + head * a.value_head;
+  t.k_row = (unsigned)a.key_row;
+  t.v_row = (unsigned)a.value_row;
+  t.row0 = p.row0;
+  t.rows = p.rows;
+  t.group = group;
+  t.first_limit = p.first_limit;
+  t.causal = true;
+  t.begin = 0;
+  t.end = p.keys;
+  Sink<Q> sink{};
+  if (splits == 1) {
+    sink.out = static_cast<Q*>(a.output) + p.begin * a.output_row + (int64_t)head * group * a.output_head;
+    sink.o_token = a.output_row;
+    sink.o_head = a.output_head;
+  } else {
+    const int visible = clamp_int(t.limit(p.row0 + p.rows - 1), 0, p.keys);
+    const int share = ((visible + C::TR - 1) / C::TR + splits - 1) / splits * C::TR;
+    t.begin = split * share;
+    t.end = t.begin + share < visible ? t.begin + share : visible;
+    const size_t item = ((size_t)slot * a.kv_heads + head) * splits + split;
+    sink.sums = static_cast<float*>(a.workspace) + item * C::BM * (D + 2);
+    sink.marks = sink.sums + C::BM * D;
+  }
+  C::run(t, sink, a.head_size, a.scale, lds, marks);
+}
+
+// Joins `count` partial rows: sums at s0 + i * step, marks at m0 + i * m_step;
+// four channels a lane.
+struct Joined {
+  float top = -kInf, total = 0.0f;
+  f32x4 o = {};
+  __device__ void add(const float* sums, const float* marks, size_t step, size_t m_step, int count) {
+    for (int i = 0; i < count; ++i) {
+      const float m = marks[i * m_step], n = marks[i * m_step + 1];
+      if (m == -kInf && n == n) continue;
+      const f32x4 v = *reinterpret_cast<const f32x4*>(sums + i * step);
+      const float next = m > top ? m : top;
+      const float keep = top == next ? 1.0f : __builtin_amdgcn_exp2f(top - next);
+      const float weight = m == next ? 1.0f : __builtin_amdgcn_exp2f(m - next);
+      total = total * keep + n * weight;
+      o = o * keep + v * weight;
+      top = next;
+    }
+  }
+  template <typename Q>
+  __device__ void write(Q* dst) const {
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    if constexpr (std::is_same_v<Q, float>) {
+      *reinterpret_cast<f32x4*>(dst) = o * inverse;
+    } else {
+      *reinterpret_cast<uint2*>(dst) = uint2{pack2<Q>(o[0] * inverse, o[1] * inverse), pack2<Q>(o[2] * inverse, o[3] * inverse)};
+    }
+  }
+};
+
+template <typename Q, int D, int BM>
+__global__ __launch_bounds__(kThreads) void packed_join_kernel(fah_packed_attention a, int splits) {
+  const int group = a.heads / a.kv_heads, head = blockIdx.x % a.kv_heads, slot = blockIdx.x / a.kv_heads;
+  const PackedTile p = packed_tile(a, slot, group, BM);
+  constexpr int kLanes = D / 4;
+  const int chunk = threadIdx.x % kLanes;
+  if (4 * chunk >= a.head_size) return;
+  const float* sums = static_cast<const float*>(a.workspace) + ((size_t)slot * a.kv_heads + head) * splits * BM * (D + 2);
+  Q* out = static_cast<Q*>(a.output) + p.begin * a.output_row + (int64_t)head * group * a.output_head;
+  for (int r = threadIdx.x / kLanes; r < p.rows; r += kThreads / kLanes) {
+    Joined j;
+    j.add(sums + r * D + 4 * chunk, sums + BM * D + 2 * r, BM * (D + 2), BM * (D + 2), splits);
+    const int row = p.row0 + r;
+    j.write(out + (row / group) * a.output_row + (row % group) * a.output_head + 4 * chunk);
+  }
+}
+
+// ---- A shared prefix ----------------------------------------------------------------
+
+// How prefix_kernel's work is cut: prefix tiles of BM rows (a row is a sequence
+// and a head of the group) times shares of the prefix, then for every sequence
+// tiles of 32 heads times shares of its own rows.
+struct PrefixCut {
+  int tiles, shares, own_tiles, own_shares;
+  int64_t prefix_items, own_items;
+};
+
+// Partial rows: [K/V head][share][sequences * group][D + 2] of the prefix, then
+// [sequence][K/V head][own share][group][D + 2]; a row's sums, then its marks.
+template <typename Q, typename K, int D, int WR, int WK, int NK>
+__global__ __launch_bounds__(kThreads) void prefix_kernel(fah_prefix_attention a, PrefixCut cut) {
+  constexpr int kArea = std::max(Core<Q, K, D, WR, WK, NK>::kTileBytes, Core<Q, K, D, 1, 4, 32>::kTileBytes);
+  __shared__ __align__(16) unsigned char lds[4 * kArea];
+  __shared__ float marks[256];
+  const int group = a.heads / a.kv_heads;
+  float* partial = static_cast<float*>(a.workspace);
+  Task<Q, K> t;
+  Sink<Q> sink{};
+  t.q_token = a.query_sequence;
+  t.q_head = a.query_head;
+  t.group = group;
+  t.causal = false;
+  if (blockIdx.x < cut.prefix_items) {
+    using C = Core<Q, K, D, WR, WK, NK>;
+    const int head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
+    const int share_at = rest % cut.shares, tile = rest / cut.shares;
+    const int all = a.sequences * group;
+    t.q = static_cast<const Q*>(a.query) + (int64_t)head * group * a.query_head;
+    t.k = static_cast<const K*>(a.prefix_key) + head * a.prefix_key_head;
+    t.v = static_cast<const K*>(a.prefix_value) + head * a.prefix_value_head;
+    t.k_row = (unsigned)a.prefix_key_row;
+    t.v_row = (unsigned)a.prefix_value_row;
+    t.row0 = tile * C::BM;
+    t.rows = clamp_int(all - t.row0, 0, C::BM);
+    const int share = ((a.prefix + C::TR - 1) / C::TR + cut.shares - 1) / cut.shares * C::TR;
+    t.begin = share_at * share;
+    t.end = t.begin + share < a.prefix ? t.begin + share : a.prefix;
+    t.first_limit = t.end;
+    const size_t rows = ((size_t)head * cut.shares + share_at) * all;
+    sink.sums = partial + rows * (D + 2) + (size_t)t.row0 * D;
+    sink.marks = partial + rows * (D + 2) + (size_t)all * D + 2 * t.row0;
+    C::run(t, sink, a.head_size, a.scale, lds, marks);
+  } else {
+    using C = Core<Q, K, D, 1, 4, 32>;
+    const int64_t at = blockIdx.x - cut.prefix_items;
+    const int head = at % a.kv_heads;
+    int64_t rest = at / a.kv_heads;
+    const int share_at = rest % cut.own_shares;
+    rest /= cut.own_shares;
+    const int tile = rest % cut.own_tiles, s = rest / cut.own_tiles;
+    const int length = __builtin_amdgcn_readfirstlane(clamp_int(a.lengths[s], 0, a.capacity));
+    t.q = static_cast<const Q*>(a.query) + s * a.query_sequence + (int64_t)head * group * a.query_head;
+    t.k = static_cast<const K*>(a.key) + s * a.key_sequence + head * a.key_head;
+    t.v = static_cast<const K*>(a.value) + s * a.value_sequence + head * a.value_head;
+    t.k_row = (unsigned)a.key_row;
+    t.v_row = (unsigned)a.value_row;
+    t.row0 = tile * C::BM;
+    t.rows = clamp_int(group - t.row0, 0, C::BM);
+    const int share = ((length + C::TR - 1) / C::TR + cut.own_shares - 1) / cut.own_shares * C::TR;
+    t.begin = share_at * share;
+    t.end = t.begin + share < length ? t.begin + share : length;
+    t.first_limit = t.end;
+    if (cut.prefix_items == 0 && cut.own_shares == 1) {
+      sink.out = static_cast<Q*>(a.output) + s * a.output_sequence + (int64_t)head * group * a.output_head;
+      sink.o_token = a.output_sequence;
+      sink.o_head = a.output_head;
+    } else {
+      const size_t rows = (size_t)a.kv_heads * cut.shares * a.sequences * group * (cut.prefix_items ? 1 : 0) +
+                          (((size_t)s * a.kv_heads + head) * cut.own_shares + share_at) * group;
+      sink.sums = partial + rows * (D + 2) + (size_t)t.row0 * D;
+      sink.marks = partial + rows * (D + 2) + (size_t)group * D + 2 * t.row0;
+    }
+    C::run(t, sink, a.head_size, a.scale, lds, marks);
+  }
+}
+
+template <typename Q, int D>
+__global__ __launch_bounds__(kThreads) void prefix_join_kernel(fah_prefix_attention a, PrefixCut cut) {
+  constexpr int kLanes = D / 4;
+  const int group = a.heads / a.kv_heads, all = a.sequences * group;
+  const int64_t at = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+  const int chunk = threadIdx.x % kLanes;
+  if (at >= (int64_t)a.sequences * a.heads || 4 * chunk >= a.head_size) return;
+  const int s = at / a.heads, q_head = at % a.heads, head = q_head / group, g = q_head % group;
+  const float* partial = static_cast<const float*>(a.workspace);
+  Joined j;
+  if (cut.prefix_items) {
+    const size_t step = (size_t)all * (D + 2);
+    const float* from = partial + (size_t)head * cut.shares * step;
+    const int row = s * group + g;
+    j.add(from + (size_t)row * D + 4 * chunk, from + (size_t)all * D + 2 * row, step, step, cut.shares);
+    partial += (size_t)a.kv_heads * cut.shares * step;
+  }
+  const size_t step = (size_t)group * (D + 2);
+  const float* from = partial + ((size_t)s * a.kv_heads + head) * cut.own_shares * step;
+  j.add(from + (size_t)g * D + 4 * chunk, from + (size_t)group * D + 2 * g, step, step, cut.own_shares);
+  j.write(static_cast<Q*>(a.output) + s * a.output_sequence + q_head * a.output_head + 4 * chunk);
+}
+
+// ---- Launch rules -------------------------------------------------------------------
+
+constexpr int kFill = 512;  // workgroups that fill the chip
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+struct PackedCut {
+  int waves_rows;  // WR
+  int splits;
+  int64_t slots;
+};
+
+PackedCut packed_cut(const fah_packed_attention& a) {
+  const int group = a.heads / a.kv_heads;
+  const int64_t rows = (int64_t)a.query_rows * group;
+  PackedCut c;
+  c.waves_rows = (int64_t)a.longest_query * group <= 32 || ceil_div(rows, 64) * a.kv_heads < kFill / 2 ? 1
+                 : ceil_div(rows, 128) * a.kv_heads < kFill                                            ? 2
+                                                                                                       : 4;
+  const int BM = 32 * c.waves_rows;
+  c.slots = rows / BM + a.sequences;
+  const int64_t items = ceil_div(rows, BM) * a.kv_heads;
+  c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kFill / items, ceil_div(a.longest_key, 512)));
+  return c;
+}
+
+PrefixCut prefix_cut(const fah_prefix_attention& a, int* waves_rows) {
+  const int group = a.heads / a.kv_heads;
+  const int64_t rows = (int64_t)a.sequences * group;
+  *waves_rows = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  PrefixCut c{};
+  c.tiles = (int)ceil_div(rows, 32 * *waves_rows);
+  c.shares = (int)std::max<int64_t>(1, std::min<int64_t>(kFill / (c.tiles * a.kv_heads), ceil_div(a.prefix, 256)));
+  c.prefix_items = a.prefix ? (int64_t)c.tiles * a.kv_heads * c.shares : 0;
+  c.own_tiles = (int)ceil_div(group, 32);
+  const int64_t own = (int64_t)a.sequences * a.kv_heads * c.own_tiles;
+  c.own_shares = (int)std::max<int64_t>(1, std::min<int64_t>(kFill / own, ceil_div(std::min(a.longest, a.capacity), 256)));
+  c.own_items = own * c.own_shares;
+  return c;
+}
+
+int width_of(int head_size) { return head_size <= 64 ? 64 : 128; }
+
+template <typename Q, typename K, int D, int WR, int WK, int NK>
+hipError_t packed_launch(const fah_packed_attention& a, const PackedCut& c, hipStream_t s) {
+  using C = Core<Q, K, D, WR, WK, NK>;
+  auto kernel = packed_kernel<Q, K, D, WR, WK, NK>;
+  kernel<<<(unsigned)(c.slots * c.splits * a.kv_heads), kThreads, 0, s>>>(a, (int)c.slots, c.splits);
+  if (c.splits > 1)
+    packed_join_kernel<Q, D, C::BM><<<(unsigned)(c.slots * a.kv_heads), kThreads, 0, s>>>(a, c.splits);
+  return hipGetLastError();
+}
+
+template <typename Q, typename K, int D>
+hipError_t packed_typed(const fah_packed_attention& a, hipStream_t s) {
+  const PackedCut c = packed_cut(a);
+  if (c.waves_rows == 1) return packed_launch<Q, K, D, 1, 4, 32>(a, c, s);
+  if (c.waves_rows == 2) return packed_launch<Q, K, D, 2, 2, 32>(a, c, s);
+  return packed_launch<Q, K, D, 4, 1, 64>(a, c, s);
+}
+
+template <typename Q, typename K, int D, int WR, int WK, int NK>
+hipError_t prefix_launch(const fah_prefix_attention& a, const PrefixCut& c, hipStream_t s) {
+  prefix_kernel<Q, K, D, WR, WK, NK><<<(unsigned)(c.prefix_items + c.own_items), kThreads, 0, s>>>(a, c);
+  if (c.prefix_items || c.own_shares > 1)
+    prefix_join_kernel<Q, D><<<(unsigned)ceil_div((int64_t)a.sequences * a.heads, kThreads / (D / 4)), kThreads, 0, s>>>(a, c);
+  return hipGetLastError();
+}
+
+template <typename Q, typename K, int D>
+hipError_t prefix_typed(const fah_prefix_attention& a, hipStream_t s) {
+  int waves_rows;
+  const PrefixCut c = prefix_cut(a, &waves_rows);
+  if (waves_rows == 1) return prefix_launch<Q, K, D, 1, 4, 32>(a, c, s);
+  if (waves_rows == 2) return prefix_launch<Q, K, D, 2, 2, 32>(a, c, s);
+  return prefix_launch<Q, K, D, 4, 1, 64>(a, c, s);
 }
 
 }  // namespace
 
 bool attention_supported(int heads, int kv_heads, int head_size, int query_type, int cache_type) {
-  return heads / kv_heads <= 65535 && head_size % 8 == 0 && head_size <= 128 &&
+  return heads % kv_heads == 0 && head_size % 8 == 0 && head_size <= 128 &&
          ((query_type == FAH_TYPE_F32 && cache_type == FAH_TYPE_F16) ||
           (query_type == FAH_TYPE_F16 && cache_type == FAH_TYPE_F16) ||
           (query_type == FAH_TYPE_BF16 && cache_type == FAH_TYPE_BF16));
 }
 
-int64_t packed_attention_workspace(const fah_packed_attention&) { return 0; }
-int64_t prefix_attention_workspace(const fah_prefix_attention&) { return 0; }
+int64_t packed_attention_workspace(const fah_packed_attention& a) {
+  if (a.sequences == 0 || a.query_rows == 0) return 0;
+  const PackedCut c = packed_cut(a);
+  return c.splits == 1 ? 0 : c.slots * a.kv_heads * c.splits * 32 * c.waves_rows * (width_of(a.head_size) + 2) * 4;
+}
+
+int64_t prefix_attention_workspace(const fah_prefix_attention& a) {
+  if (a.sequences == 0) return 0;
+  int waves_rows;
+  const PrefixCut c = prefix_cut(a, &waves_rows);
+  if (!c.prefix_items && c.own_shares == 1) return 0;
+  const int64_t rows = ((c.prefix_items ? c.shares : 0) + c.own_shares) * (int64_t)a.sequences * a.heads;
+  return rows * (width_of(a.head_size) + 2) * 4;
+}
 
 hipError_t launch_packed_attention(const fah_packed_attention& a, hipStream_t s) {
-  const dim3 grid(a.query_rows, a.heads);
-  if (a.query_type == FAH_TYPE_F32) packed_rows_kernel<float, _Float16><<<grid, 64, 0, s>>>(a);
-  else if (a.query_type == FAH_TYPE_F16) packed_rows_kernel<_Float16, _Float16><<<grid, 64, 0, s>>>(a);
-  else packed_rows_kernel<__bf16, __bf16><<<grid, 64, 0, s>>>(a);
-  return hipGetLastError();
+  const bool wide = width_of(a.head_size) == 128;
+  if (a.query_type == FAH_TYPE_F32)
+    return wide ? packed_typed<float, _Float16, 128>(a, s) : packed_typed<float, _Float16, 64>(a, s);
+  if (a.query_type == FAH_TYPE_F16)
+    return wide ? packed_typed<_Float16, _Float16, 128>(a, s) : packed_typed<_Float16, _Float16, 64>(a, s);
+  return wide ? packed_typed<__bf16, __bf16, 128>(a, s) : packed_typed<__bf16, __bf16, 64>(a, s);
 }
 
 hipError_t launch_prefix_attention(const fah_prefix_attention& a, hipStream_t s) {
-  const dim3 grid(a.sequences, a.heads);
-  if (a.query_type == FAH_TYPE_F32) prefix_rows_kernel<float, _Float16><<<grid, 64, 0, s>>>(a);
-  else if (a.query_type == FAH_TYPE_F16) prefix_rows_kernel<_Float16, _Float16><<<grid, 64, 0, s>>>(a);
-  else prefix_rows_kernel<__bf16, __bf16><<<grid, 64, 0, s>>>(a);
-  return hipGetLastError();
+  const bool wide = width_of(a.head_size) == 128;
+  if (a.query_type == FAH_TYPE_F32)
+    return wide ? prefix_typed<float, _Float16, 128>(a, s) : prefix_typed<float, _Float16, 64>(a, s);
+  if (a.query_type == FAH_TYPE_F16)
+    return wide ? prefix_typed<_Float16, _Float16, 128>(a, s) : prefix_typed<_Float16, _Float16, 64>(a, s);
+  return wide ? prefix_typed<__bf16, __bf16, 128>(a, s) : prefix_typed<__bf16, __bf16, 64>(a, s);
 }
 
 }  // namespace fah
