@@ -1,86 +1,208 @@
 // Logits under penalties for repeated tokens, biases and grammar masks, and the
 // greedy choice after them (fah_logits_adjust of the C ABI).
 //
-// Two launches. logits_kernel: a workgroup takes kChunk tokens of one row. It
-// clears a table of one pair of words per token in LDS, scans the row's history
-// and bias list once (each chunk scans them whole: a few KB, from the L2) and
-// notes the entries that fall into its tokens with integer LDS atomics, whose
-// result does not depend on their order: the word `seen` is the count behind
-// the prompt and, in bit 31, whether the token stands in the history at all;
-// `entry` is the last list entry of the token's bias plus one. Then it streams
-// its logits through registers once, 16 bytes a lane, and keeps each lane's
-// largest written value. choice_kernel takes the largest over a row's chunks.
+// logits_kernel: a workgroup takes some chunks of one row's tokens. It holds the
+// row's lists in registers and requests a chunk's logits, 16 bytes a lane, while
+// it notes what the lists say of the chunk before in a table in LDS: they name
+// few tokens, so the stream itself only carries the mask, the running maximum
+// and one bit a token that asks for the table. choice_kernel takes the largest
+// over a row's workgroups.
 #include "fah_device.h"
 #include "fah_internal.h"
+
+#include <algorithm>
 
 namespace fah {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 1024;
+constexpr float kInf = __builtin_inff();
 
+// Values of T in 16 bytes, and back.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void logits_kernel(fah_logits_adjust a, unsigned long long* keys) {
-  __shared__ unsigned seen[kChunk], entry[kChunk];
+struct alignas(16) Vec {
+  static constexpr int kCount = 16 / sizeof(T);
+  T v[kCount];
+};
+
+// This thread's share of a list, every kThreads-th entry: the first kHeld in
+// registers, requested together, the others when they are looked at.
+template <int kHeld>
+struct List {
+  const int* at;
+  int count, held[kHeld];
+  __device__ __forceinline__ List(const int* list, int n) : at(list), count(n) {
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int i = threadIdx.x + k * kThreads;
+      held[k] = i < count ? at[i] : -1;
+    }
+  }
+  // f(token, entry)
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) f(held[k], (int)threadIdx.x + k * kThreads);
+    for (int i = threadIdx.x + kHeld * kThreads; i < count; i += kThreads) f(at[i], i);
+  }
+};
+
+__device__ __forceinline__ int bounded(const int* counts, int row, int capacity) {
+  const int n = counts ? counts[row] : capacity;
+  return n < 0 ? 0 : n < capacity ? n : capacity;
+}
+
+// Tokens of a row are counted from the 16-byte boundary at or before its first
+// logit: place u = token + lead, so that groups of Vec::kCount places are whole
+// 16-byte loads whatever the row's alignment. A workgroup takes `run` chunks of
+// kChunk places, a group a thread, the next chunk's on their way meanwhile.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void logits_kernel(fah_logits_adjust a, int run, unsigned long long* keys) {
+  constexpr int V = Vec<T>::kCount, kChunk = kThreads * V;
+  // What the lists say of a place: `seen` the count behind the prompt and in
+  // bit 31 whether it is in the history at all; `entry` its last bias entry plus
+  // one; `named` a bit for a place in either. Integer atomics: no order changes
+  // the result.
+  struct Table {
+    unsigned seen[kChunk], entry[kChunk], named[kChunk / 32];
+  };
+  __shared__ __align__(16) Table table;
   __shared__ unsigned long long part[kThreads / kWave];
-  const int row = blockIdx.y, first = blockIdx.x * kChunk, tid = threadIdx.x;
-  const int tokens = a.vocab - first < kChunk ? a.vocab - first : kChunk;
-  for (int i = tid; i < kChunk; i += kThreads) seen[i] = entry[i] = 0;
-  __syncthreads();
-  if (a.history_capacity) {
-    const int* list = a.history + row * a.history_stride;
-    int n = a.history_counts ? a.history_counts[row] : a.history_capacity;
-    n = n < a.history_capacity ? n : a.history_capacity;
-    const int prompt = a.prompt_counts ? a.prompt_counts[row] : 0;
-    for (int i = tid; i < n; i += kThreads) {
-      const unsigned t = (unsigned)list[i] - (unsigned)first;
-      if (list[i] >= 0 && t < (unsigned)tokens) {
-        atomicOr(&seen[t], 0x80000000u);
-        if (i >= prompt) atomicAdd(&seen[t], 1u);
-      }
-    }
-  }
-  if (a.bias_capacity) {
-    const int* list = a.bias_tokens + row * a.bias_stride;
-    int n = a.bias_counts ? a.bias_counts[row] : a.bias_capacity;
-    n = n < a.bias_capacity ? n : a.bias_capacity;
-    for (int i = tid; i < n; i += kThreads) {
-      const unsigned t = (unsigned)list[i] - (unsigned)first;
-      if (list[i] >= 0 && t < (unsigned)tokens) atomicMax(&entry[t], (unsigned)i + 1u);
-    }
-  }
-  __syncthreads();
-  const float repetition = a.repetition ? a.repetition[row] : 1.0f;
-  const float presence = a.presence ? a.presence[row] : 0.0f;
-  const float frequency = a.frequency ? a.frequency[row] : 0.0f;
+  const int row = blockIdx.y, tid = threadIdx.x;
+  const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
+  T* out = static_cast<T*>(a.output) + row * a.output_stride;
+  const int lead = (int)(reinterpret_cast<uintptr_t>(in) % 16 / sizeof(T));
+  const bool out_alike = reinterpret_cast<uintptr_t>(out) % 16 / sizeof(T) == (unsigned)lead;
   const uint32_t* mask = nullptr;
   if (a.mask_rows) {
     const int m = a.mask_index ? a.mask_index[row] : a.mask_rows == 1 ? 0 : row;
     if (m >= 0 && m < a.mask_rows) mask = a.masks + m * a.mask_stride;
   }
-  const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride + first;
-  T* out = static_cast<T*>(a.output) + row * a.output_stride + first;
-  unsigned long long best = 0;
-  for (int i = tid; i < tokens; i += kThreads) {
-    float x = (float)in[i];
-    const unsigned w = seen[i], e = entry[i];
-    if (w) x = x > 0.0f ? x / repetition : x * repetition;
-    const unsigned n = w & 0x7fffffffu;
-    if (n) {
-      x = x - frequency * (float)n;
-      x = x - presence;
+
+  // A thread's logits and mask bits of a chunk; t: the token of its first place.
+  struct Group {
+    Vec<T> x;
+    uint32_t low, high;
+  };
+  auto load = [&](int t) {
+    Group g{};
+    g.low = g.high = ~0u;
+    if (t >= 0 && t + V <= a.vocab) {
+      g.x = *reinterpret_cast<const Vec<T>*>(in + t);
+      if (mask) {
+        g.low = mask[t >> 5];
+        g.high = mask[(t + V - 1) >> 5];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) g.x.v[e] = t + e >= 0 && t + e < a.vocab ? in[t + e] : (T)0.0f;
+      if (mask && t + V > 0 && t < a.vocab) {
+        g.low = mask[t >= 0 ? t >> 5 : 0];
+        g.high = mask[(t + V <= a.vocab ? t + V - 1 : a.vocab - 1) >> 5];
+      }
     }
-    if (e) x = x + a.bias_values[row * a.bias_stride + (e - 1)];
-    if (mask && !(mask[(first + i) >> 5] >> ((first + i) & 31) & 1u)) x = -__builtin_inff();
-    const T y = (T)x;
-    out[i] = y;
-    if ((float)y > -__builtin_inff()) {
-      const unsigned long long key = greedy_key((float)y, (uint32_t)(first + i));
-      best = key > best ? key : best;
+    return g;
+  };
+  // Bit e: token t + e is allowed (low: the mask's word with token t, or with
+  // token 0; high: the one with the group's last token).
+  auto allowed = [&](const Group& g, int t) {
+    const int shift = t & 31;
+    if (t < 0) return g.low << -t;
+    return shift + V > 32 ? g.low >> shift | g.high << (32 - shift) : g.low >> shift;
+  };
+  int first = (int)blockIdx.x * run * kChunk - lead;  // token of the chunk's place 0
+  Group next = load(first + tid * V);
+
+  const int history_count = a.history_capacity ? bounded(a.history_counts, row, a.history_capacity) : 0;
+  const int bias_count = a.bias_capacity ? bounded(a.bias_counts, row, a.bias_capacity) : 0;
+  const bool listed = history_count + bias_count > 0;
+  const int prompt = a.prompt_counts ? a.prompt_counts[row] : 0;
+  const float repetition = a.repetition ? a.repetition[row] : 1.0f;
+  const float presence = a.presence ? a.presence[row] : 0.0f;
+  const float frequency = a.frequency ? a.frequency[row] : 0.0f;
+  const float* bias = a.bias_values + row * a.bias_stride;
+  const List<4> history(a.history + row * a.history_stride, history_count);
+  const List<2> biases(a.bias_tokens + row * a.bias_stride, bias_count);
+  auto adjust = [&](float v, int u) {
+    const unsigned w = table.seen[u], e = table.entry[u], n = w & 0x7fffffffu;
+    if (w) v = v > 0.0f ? v / repetition : v * repetition;
+    if (n) {
+      v = v - frequency * (float)n;
+      v = v - presence;
+    }
+    return e ? v + bias[e - 1] : v;
+  };
+
+  float top = -kInf;  // NaN and -inf never replace it
+  int at = -1;
+  for (int c = 0; c < run && first < a.vocab; ++c, first += kChunk) {
+    const int t = first + tid * V;
+    Group g = next;
+    if (c + 1 < run) next = load(t + kChunk);
+    uint32_t bits = 0;
+    if (listed) {
+      auto place = [&](int token) {
+        const unsigned u = (unsigned)(token - first);
+        return token >= 0 && token < a.vocab && u < (unsigned)kChunk ? (int)u : -1;
+      };
+      for (int i = tid; i < (int)sizeof(Table) / 16; i += kThreads) reinterpret_cast<uint4*>(&table)[i] = uint4{0, 0, 0, 0};
+      lds_barrier();
+      history.each([&](int token, int i) {
+        const int u = place(token);
+        if (u < 0) return;
+        atomicOr(&table.named[u >> 5], 1u << (u & 31));
+        atomicOr(&table.seen[u], 0x80000000u);
+        if (i >= prompt) atomicAdd(&table.seen[u], 1u);
+      });
+      biases.each([&](int token, int i) {
+        const int u = place(token);
+        if (u < 0) return;
+        atomicOr(&table.named[u >> 5], 1u << (u & 31));
+        atomicMax(&table.entry[u], (unsigned)i + 1);
+      });
+      lds_barrier();
+      bits = table.named[tid * V >> 5] >> (tid * V & 31) & ((1u << V) - 1);
+      if (bits) {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (bits >> e & 1) g.x.v[e] = (T)adjust((float)g.x.v[e], tid * V + e);
+      }
+      lds_barrier();  // before the next chunk clears the table
+    }
+    const uint32_t open = allowed(g, t);
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (!(open >> e & 1)) g.x.v[e] = (T)-kInf;
+    if (t >= 0 && t + V <= a.vocab) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float y = (float)g.x.v[e];
+        if (y > top) {
+          top = y;
+          at = t + e;
+        }
+      }
+      if (out_alike) {
+        *reinterpret_cast<Vec<T>*>(out + t) = g.x;
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) out[t + e] = g.x.v[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (t + e >= 0 && t + e < a.vocab) {
+          const float y = (float)g.x.v[e];
+          out[t + e] = g.x.v[e];
+          if (y > top) {
+            top = y;
+            at = t + e;
+          }
+        }
     }
   }
   if (!keys) return;
-  best = wave_max_u64(best);
+  unsigned long long best = wave_max_u64(at < 0 ? 0ull : greedy_key(top, (uint32_t)at));
   if (tid % kWave == 0) part[tid / kWave] = best;
   __syncthreads();
   if (tid == 0) {
@@ -99,21 +221,34 @@ __global__ __launch_bounds__(kWave) void choice_kernel(const unsigned long long*
   if (threadIdx.x == 0) tokens[blockIdx.x] = best ? (int)greedy_index(best) : -1;
 }
 
-int chunks_of(const fah_logits_adjust& a) { return (a.vocab + kChunk - 1) / kChunk; }
+// Chunks a workgroup takes, and the workgroups of a row.
+struct ChoiceCut {
+  int run, groups;
+};
+
+constexpr int kGroups = 4096;
+
+ChoiceCut choice_cut(const fah_logits_adjust& a) {
+  const int V = a.type == FAH_TYPE_F32 ? 4 : 8;
+  const int64_t chunks = ((int64_t)a.vocab + V - 1 + kThreads * V - 1) / (kThreads * V);
+  const int run = (int)std::max<int64_t>(1, std::min<int64_t>(chunks * a.rows / kGroups, 8));
+  return {run, (int)((chunks + run - 1) / run)};
+}
 
 }  // namespace
 
 int64_t logits_adjust_workspace(const fah_logits_adjust& a) {
-  return a.tokens && a.rows > 0 ? (int64_t)a.rows * chunks_of(a) * 8 : 0;
+  return a.tokens && a.rows > 0 ? (int64_t)a.rows * choice_cut(a).groups * 8 : 0;
 }
 
 hipError_t launch_logits_adjust(const fah_logits_adjust& a, hipStream_t s) {
-  const dim3 grid(chunks_of(a), a.rows);
+  const ChoiceCut c = choice_cut(a);
+  const dim3 grid(c.groups, a.rows);
   auto* keys = a.tokens ? static_cast<unsigned long long*>(a.workspace) : nullptr;
-  if (a.type == FAH_TYPE_F32) logits_kernel<float><<<grid, kThreads, 0, s>>>(a, keys);
-  else if (a.type == FAH_TYPE_F16) logits_kernel<_Float16><<<grid, kThreads, 0, s>>>(a, keys);
-  else logits_kernel<__bf16><<<grid, kThreads, 0, s>>>(a, keys);
-  if (keys) choice_kernel<<<a.rows, kWave, 0, s>>>(keys, grid.x, a.tokens);
+  if (a.type == FAH_TYPE_F32) logits_kernel<float><<<grid, kThreads, 0, s>>>(a, c.run, keys);
+  else if (a.type == FAH_TYPE_F16) logits_kernel<_Float16><<<grid, kThreads, 0, s>>>(a, c.run, keys);
+  else logits_kernel<__bf16><<<grid, kThreads, 0, s>>>(a, c.run, keys);
+  if (keys) choice_kernel<<<a.rows, kWave, 0, s>>>(keys, c.groups, a.tokens);
   return hipGetLastError();
 }
 
