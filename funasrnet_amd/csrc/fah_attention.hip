@@ -101,6 +101,14 @@ __device__ __forceinline__ void load_lds(const void* from, unsigned to) {
 // follows: reads of LDS may move up to it but not before it.
 __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
+// All but the last N loads are done; reads of LDS stay behind it.
+template <int N>
+__device__ __forceinline__ void wait_loads_but() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// This wave's reads of LDS are done: their place may be loaded again.
+__device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 __device__ __forceinline__ unsigned lds_address(const void* p) {
   return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }
@@ -198,6 +206,9 @@ template <typename Q, typename K, int D, int WR, int WK, int NK>
 struct Core {
   static constexpr int BM = 32 * WR, TR = WK * NK;
   static constexpr int kTileBytes = TR * 2 * D;        // keys, or values
+  // One group of rows: each wave's keys and values are its own, in one buffer.
+  // Several groups share them, in two.
+  static constexpr int kBuffers = WR == 1 ? 1 : 2, kLds = kBuffers * 2 * kTileBytes;
   static constexpr bool kSplit = std::is_same_v<Q, float>;
   static constexpr int kSteps = D / 16;
 
@@ -205,7 +216,7 @@ struct Core {
   // sums. marks: [4][32][2].
   __device__ static void run(const Task<Q, K>& t, const Sink<Q>& sink, int size, float scale, unsigned char* lds,
                              float* marks) {
-    static_assert(kTileBytes >= 32 * D * 4);
+    static_assert(kLds >= 4 * 32 * D * 4);
     using T = Tile<D>;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
     const int wr = wave / WK, wk = wave % WK;
@@ -219,19 +230,27 @@ struct Core {
     const int last = t.end - 1;
 
     if (D != size) {
-      for (int i = tid; i < 4 * kTileBytes / 16; i += kThreads) reinterpret_cast<uint4*>(lds)[i] = uint4{0, 0, 0, 0};
+      for (int i = tid; i < kLds / 16; i += kThreads) reinterpret_cast<uint4*>(lds)[i] = uint4{0, 0, 0, 0};
       __syncthreads();
     }
-    // With one group of rows a wave loads the keys that it takes itself.
     constexpr int kOwn = WR == 1 ? NK : TR, kLoaders = WR == 1 ? 1 : 4;
     const int own = WR == 1 ? wave * NK : 0, loader = WR == 1 ? 0 : wave;
-    const Loader<K, D, kOwn, kLoaders, false> keys(lds + own * T::kRowBytes, t.k_row, loader);
-    const Loader<K, D, kOwn, kLoaders, true> values(lds + kTileBytes + own * T::kRowBytes, t.v_row, loader);
-    auto load = [&](int buffer, int key) {
-      keys.load(t.k, t.k_row, key + own, last, buffer * 2 * kTileBytes, size);
-      values.load(t.v, t.v_row, key + own, last, buffer * 2 * kTileBytes, size);
+    using KeyLoader = Loader<K, D, kOwn, kLoaders, false>;
+    using ValueLoader = Loader<K, D, kOwn, kLoaders, true>;
+    const KeyLoader key_loader(lds + own * T::kRowBytes, t.k_row, loader);
+    const ValueLoader value_loader(lds + kTileBytes + own * T::kRowBytes, t.v_row, loader);
+    auto load_keys = [&](int buffer, int key) {
+      key_loader.load(t.k, t.k_row, key, last, buffer * 2 * kTileBytes, size);
     };
-    if (t.begin < end) load(0, t.begin);
+    auto load_values = [&](int buffer, int key) {
+      value_loader.load(t.v, t.v_row, key, last, buffer * 2 * kTileBytes, size);
+    };
+    // The wave's first key, and the end of those that its rows see.
+    const int wave_begin = t.begin + wk * NK, wave_end = lim_high;
+    if (WR == 1 ? wave_begin < wave_end : t.begin < end) {
+      load_keys(0, t.begin + own);
+      load_values(0, t.begin + own);
+    }
 
     // Queries: the B operand, lane (row col, channels 16 s + 8 half ..). fp32
     // queries are scaled by a power of two to below 2^14 and split into two
@@ -292,10 +311,9 @@ struct Core {
     const int value_at = (wk * NK + 4 * half + vi / 4) * T::kRowBytes + (vi & 1) * 8;
     const int value_sw = T::value_swizzle(vi / 4), value_chunk = 2 * vg + ((vi & 3) >> 1);
 
-    auto compute = [&](int buffer, int key0) {
+    f32x16 s[NK / 32];
+    auto score = [&](int buffer) {
       const unsigned char* kt = lds + buffer * 2 * kTileBytes;
-      const unsigned char* vt = kt + kTileBytes;
-      f32x16 s[NK / 32];
 #pragma unroll
       for (int b = 0; b < NK / 32; ++b) s[b] = f32x16{};
 #pragma unroll
@@ -306,6 +324,9 @@ struct Core {
           s[b] = mfma<K>(kf, qf[0][step], s[b]);
           if constexpr (kSplit) s[b] = mfma<K>(kf, qf[kSplit ? 1 : 0][step], s[b]);
         }
+    };
+    // Scores to weights, in place.
+    auto weigh = [&](int key0) {
       if (key0 + NK > lim_low) {
         masked = true;
         const int room = lim - key0 - 4 * half;
@@ -336,6 +357,9 @@ struct Core {
           s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, base));
           total += s[b][i];
         }
+    };
+    auto collect = [&](int buffer) {
+      const unsigned char* vt = lds + buffer * 2 * kTileBytes + kTileBytes;
 #pragma unroll
       for (int step = 0; step < NK / 16; ++step) {
         // The B operand of 16 keys: a lane's eight weights as they are; the
@@ -365,17 +389,44 @@ struct Core {
       }
     };
 
-    // One pass a buffer. The barrier: this buffer's tile is here, and the other
-    // one's readers are done.
-    auto pass = [&](int buffer, int key) {
+    if constexpr (WR == 1) {
+      // The next keys are on their way from the moment these are read, the next
+      // values likewise: one buffer, and no wave waits for another.
       wait_loads();
-      __syncthreads();
-      if (key + TR < end) load(buffer ^ 1, key + TR);
-      if (key + wk * NK < lim_high) compute(buffer, key + wk * NK);
-    };
-    for (int key = t.begin; key < end; key += 2 * TR) {
-      pass(0, key);
-      if (key + TR < end) pass(1, key + TR);
+      for (int key = wave_begin; key < wave_end; key += TR) {
+        const bool more = key + TR < wave_end;
+        wait_loads_but<ValueLoader::kLoads>();
+        score(0);
+        wait_reads();
+        if (more) load_keys(0, key + TR);
+        weigh(key);
+        if (more) wait_loads_but<KeyLoader::kLoads>();
+        else wait_loads_but<0>();
+        collect(0);
+        wait_reads();
+        if (more) load_values(0, key + TR);
+      }
+    } else {
+      // One pass a buffer. The barrier: this buffer's tile is here, and the
+      // other one's readers are done.
+      auto pass = [&](int buffer, int key) {
+        wait_loads();
+        __syncthreads();
+        if (key + TR < end) {
+          load_keys(buffer ^ 1, key + TR);
+          load_values(buffer ^ 1, key + TR);
+        }
+        const int mine = key + wk * NK;
+        if (mine < wave_end) {
+          score(buffer);
+          weigh(mine);
+          collect(buffer);
+        }
+      };
+      for (int key = t.begin; key < end; key += 2 * TR) {
+        pass(0, key);
+        if (key + TR < end) pass(1, key + TR);
+      }
     }
     total += other_half(total);
 
@@ -500,7 +551,7 @@ __device__ __forceinline__ PackedTile packed_tile(const fah_packed_attention& a,
 template <typename Q, typename K, int D, int WR, int WK, int NK>
 __global__ __launch_bounds__(kThreads) void packed_kernel(fah_packed_attention a, int slots, int splits) {
   using C = Core<Q, K, D, WR, WK, NK>;
-  __shared__ __align__(16) unsigned char lds[4 * C::kTileBytes];
+  __shared__ __align__(16) unsigned char lds[C::kLds];
   __shared__ float marks[256];
   const int group = a.heads / a.kv_heads, head = blockIdx.x % a.kv_heads;
   const int rest = blockIdx.x / a.kv_heads, split = rest % splits, slot = slots - 1 - rest / splits;
@@ -538,21 +589,38 @@ __global__ __launch_bounds__(kThreads) void packed_kernel(fah_packed_attention a
   C::run(t, sink, a.head_size, a.scale, lds, marks);
 }
 
-// Joins `count` partial rows: sums at s0 + i * step, marks at m0 + i * m_step;
-// four channels a lane.
+// Joins partial rows by groups of D / 4 lanes, four channels a lane: `count`
+// partial sums, sums at s0 + i * step and marks at m0 + i * step. The marks are
+// read by a lane each and shared, so that every load stands alone.
+template <int D>
 struct Joined {
+  static constexpr int kLanes = D / 4;
   float top = -kInf, total = 0.0f;
   f32x4 o = {};
-  __device__ void add(const float* sums, const float* marks, size_t step, size_t m_step, int count) {
-    for (int i = 0; i < count; ++i) {
-      const float m = marks[i * m_step], n = marks[i * m_step + 1];
-      if (m == -kInf && n == n) continue;
-      const f32x4 v = *reinterpret_cast<const f32x4*>(sums + i * step);
-      const float next = m > top ? m : top;
-      const float keep = top == next ? 1.0f : __builtin_amdgcn_exp2f(top - next);
-      const float weight = m == next ? 1.0f : __builtin_amdgcn_exp2f(m - next);
-      total = total * keep + n * weight;
-      o = o * keep + v * weight;
+  __device__ __forceinline__ void add(const float* sums, const float* marks, size_t step, int count) {
+    const int lane = threadIdx.x % kLanes;
+    for (int first = 0; first < count; first += kLanes) {
+      const int n = count - first < kLanes ? count - first : kLanes;
+      float m = -kInf, w = 0.0f;
+      if (lane < n) {
+        m = marks[(first + lane) * step];
+        w = marks[(first + lane) * step + 1];
+      }
+      float next = fmaxf(top, m);
+      for (int x = kLanes / 2; x >= 1; x >>= 1) next = fmaxf(next, __shfl_xor(next, x, kLanes));
+      // A partial row that saw nothing counts as nothing, unless its total is NaN.
+      const float weight = m == next && m != -kInf ? 1.0f : m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - next);
+      const float keep = top == -kInf || top == next ? 1.0f : __builtin_amdgcn_exp2f(top - next);
+      float sum = w == w ? weight * w : w;
+      for (int x = kLanes / 2; x >= 1; x >>= 1) sum += __shfl_xor(sum, x, kLanes);
+      total = total * keep + sum;
+      o *= keep;
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const float wi = __shfl(weight, i, kLanes);
+        const f32x4 v = *reinterpret_cast<const f32x4*>(sums + (first + i) * step);
+        o += wi == 0.0f ? f32x4{} : v * wi;
+      }
       top = next;
     }
   }
@@ -573,14 +641,13 @@ __global__ __launch_bounds__(kThreads) void packed_join_kernel(fah_packed_attent
   const PackedTile p = packed_tile(a, slot, group, BM);
   constexpr int kLanes = D / 4;
   const int chunk = threadIdx.x % kLanes;
-  if (4 * chunk >= a.head_size) return;
   const float* sums = static_cast<const float*>(a.workspace) + ((size_t)slot * a.kv_heads + head) * splits * BM * (D + 2);
   Q* out = static_cast<Q*>(a.output) + p.begin * a.output_row + (int64_t)head * group * a.output_head;
   for (int r = threadIdx.x / kLanes; r < p.rows; r += kThreads / kLanes) {
-    Joined j;
-    j.add(sums + r * D + 4 * chunk, sums + BM * D + 2 * r, BM * (D + 2), BM * (D + 2), splits);
+    Joined<D> j;
+    j.add(sums + r * D + 4 * chunk, sums + BM * D + 2 * r, BM * (D + 2), splits);
     const int row = p.row0 + r;
-    j.write(out + (row / group) * a.output_row + (row % group) * a.output_head + 4 * chunk);
+    if (4 * chunk < a.head_size) j.write(out + (row / group) * a.output_row + (row % group) * a.output_head + 4 * chunk);
   }
 }
 
@@ -598,8 +665,8 @@ struct PrefixCut {
 // [sequence][K/V head][own share][group][D + 2]; a row's sums, then its marks.
 template <typename Q, typename K, int D, int WR, int WK, int NK>
 __global__ __launch_bounds__(kThreads) void prefix_kernel(fah_prefix_attention a, PrefixCut cut) {
-  constexpr int kArea = std::max(Core<Q, K, D, WR, WK, NK>::kTileBytes, Core<Q, K, D, 1, 4, 32>::kTileBytes);
-  __shared__ __align__(16) unsigned char lds[4 * kArea];
+  constexpr int kLds = std::max(Core<Q, K, D, WR, WK, NK>::kLds, Core<Q, K, D, 1, 4, 32>::kLds);
+  __shared__ __align__(16) unsigned char lds[kLds];
   __shared__ float marks[256];
   const int group = a.heads / a.kv_heads;
   float* partial = static_cast<float*>(a.workspace);
@@ -669,21 +736,21 @@ __global__ __launch_bounds__(kThreads) void prefix_join_kernel(fah_prefix_attent
   const int group = a.heads / a.kv_heads, all = a.sequences * group;
   const int64_t at = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
   const int chunk = threadIdx.x % kLanes;
-  if (at >= (int64_t)a.sequences * a.heads || 4 * chunk >= a.head_size) return;
+  if (at >= (int64_t)a.sequences * a.heads) return;
   const int s = at / a.heads, q_head = at % a.heads, head = q_head / group, g = q_head % group;
   const float* partial = static_cast<const float*>(a.workspace);
-  Joined j;
+  Joined<D> j;
   if (cut.prefix_items) {
     const size_t step = (size_t)all * (D + 2);
     const float* from = partial + (size_t)head * cut.shares * step;
     const int row = s * group + g;
-    j.add(from + (size_t)row * D + 4 * chunk, from + (size_t)all * D + 2 * row, step, step, cut.shares);
+    j.add(from + (size_t)row * D + 4 * chunk, from + (size_t)all * D + 2 * row, step, cut.shares);
     partial += (size_t)a.kv_heads * cut.shares * step;
   }
   const size_t step = (size_t)group * (D + 2);
   const float* from = partial + ((size_t)s * a.kv_heads + head) * cut.own_shares * step;
-  j.add(from + (size_t)g * D + 4 * chunk, from + (size_t)group * D + 2 * g, step, step, cut.own_shares);
-  j.write(static_cast<Q*>(a.output) + s * a.output_sequence + q_head * a.output_head + 4 * chunk);
+  j.add(from + (size_t)g * D + 4 * chunk, from + (size_t)group * D + 2 * g, step, cut.own_shares);
+  if (4 * chunk < a.head_size) j.write(static_cast<Q*>(a.output) + s * a.output_sequence + q_head * a.output_head + 4 * chunk);
 }
 
 // ---- Launch rules -------------------------------------------------------------------
