@@ -46,32 +46,39 @@ __device__ __forceinline__ float other_half(float v) {
   return u2f(threadIdx.x & 32 ? r[0] : r[1]);
 }
 
-// What one workgroup attends: BM rows (of one K/V head: the row r is token r /
-// group, query head r % group of the head's group) over the keys [begin, end).
+// What one workgroup attends: `rows` rows of one K/V head over the keys
+// [begin, end). A row is a token and one of the group's query heads, heads
+// first; the first row is head head0 of token 0.
 template <typename Q, typename K>
 struct Task {
   const Q* q;                // token 0, the K/V head's first query head
   int64_t q_token, q_head;   // strides
   const K *k, *v;            // key 0
   unsigned k_row, v_row;     // strides
-  int row0, rows, group;     // rows row0 .. row0 + rows - 1
+  int rows, group, head0;
+  float group_inverse;
   int begin, end;            // keys
   int first_limit;           // token 0 sees the keys below this; per token one more if causal
   bool causal;
-  __device__ int limit(int row) const {
-    const int64_t n = (int64_t)first_limit + (causal ? row / group : 0);
-    return n < end ? (int)n : end;
+  // Row r's token and head. (r + head0 is below 2^20: the product is within a
+  // quarter of the exact quotient, which is at least half a step from a whole
+  // number's edge.)
+  __device__ __forceinline__ int token(int r) const { return (int)((float)(r + head0) * group_inverse + 0.5f * group_inverse); }
+  __device__ __forceinline__ int head(int r) const { return r + head0 - token(r) * group; }
+  __device__ __forceinline__ int limit(int r) const {
+    const int n = causal ? first_limit + token(r) : first_limit;
+    return n < end ? n : end;
   }
-  __device__ const Q* query(int row) const { return q + (row / group) * q_token + (row % group) * q_head; }
+  __device__ __forceinline__ const Q* query(int r) const { return q + token(r) * q_token + head(r) * q_head; }
 };
 
-// Where it goes: the finished rows, or partial sums for combine_*: per row
-// [size] sums, then the reference and the total.
+// Where it goes: the finished rows, or partial ones for a join: sums, each
+// row's reference (a power of two) and total.
 template <typename Q>
 struct Sink {
   Q* out;                    // token 0, the K/V head's first query head; null: partial
   int64_t o_token, o_head;
-  float* sums;               // of row row0: [rows][D]
+  float* sums;               // [rows][D]
   float* marks;              // [rows][2]
 };
 
@@ -213,7 +220,8 @@ struct Core {
   static constexpr int kSteps = D / 16;
 
   // lds: two buffers of a key tile and a value tile; at the end the waves'
-  // sums. marks: [4][32][2].
+  // sums. marks: [4][32][2], then
+  // [128][2].
   __device__ static void run(const Task<Q, K>& t, const Sink<Q>& sink, int size, float scale, unsigned char* lds,
                              float* marks) {
     static_assert(kLds >= 4 * 32 * D * 4);
@@ -222,11 +230,11 @@ struct Core {
     const int wr = wave / WK, wk = wave % WK;
     const int my_row = wr * 32 + col;
     const bool valid = my_row < t.rows;
-    const int lim = valid ? t.limit(t.row0 + my_row) : 0;
+    const int lim = valid ? t.limit(my_row) : 0;
     const int wave_rows = clamp_int(t.rows - wr * 32, 0, 32);
-    const int lim_low = wave_rows ? t.limit(t.row0 + wr * 32) : 0;
-    const int lim_high = wave_rows ? t.limit(t.row0 + wr * 32 + wave_rows - 1) : 0;
-    const int end = t.rows ? t.limit(t.row0 + t.rows - 1) : 0;  // of the workgroup
+    const int lim_low = wave_rows ? t.limit(wr * 32) : 0;
+    const int lim_high = wave_rows ? t.limit(wr * 32 + wave_rows - 1) : 0;
+    const int end = t.limit(t.rows - 1);  // of the workgroup
     const int last = t.end - 1;
 
     if (D != size) {
@@ -239,18 +247,8 @@ struct Core {
     using ValueLoader = Loader<K, D, kOwn, kLoaders, true>;
     const KeyLoader key_loader(lds + own * T::kRowBytes, t.k_row, loader);
     const ValueLoader value_loader(lds + kTileBytes + own * T::kRowBytes, t.v_row, loader);
-    auto load_keys = [&](int buffer, int key) {
-      key_loader.load(t.k, t.k_row, key, last, buffer * 2 * kTileBytes, size);
-    };
-    auto load_values = [&](int buffer, int key) {
-      value_loader.load(t.v, t.v_row, key, last, buffer * 2 * kTileBytes, size);
-    };
     // The wave's first key, and the end of those that its rows see.
     const int wave_begin = t.begin + wk * NK, wave_end = lim_high;
-    if (WR == 1 ? wave_begin < wave_end : t.begin < end) {
-      load_keys(0, t.begin + own);
-      load_values(0, t.begin + own);
-    }
 
     // Queries: the B operand, lane (row col, channels 16 s + 8 half ..). fp32
     // queries are scaled by a power of two to below 2^14 and split into two
@@ -258,7 +256,7 @@ struct Core {
     s16x8 qf[kSplit ? 2 : 1][kSteps];
     float c = scale * kLog2e;
     {
-      const Q* q = t.query(t.row0 + (valid ? my_row : 0));
+      const Q* q = t.query(valid ? my_row : 0);
       if constexpr (kSplit) {
         f32x4 x[kSteps][2];
         float most = 0.0f;
@@ -312,8 +310,8 @@ struct Core {
     const int value_sw = T::value_swizzle(vi / 4), value_chunk = 2 * vg + ((vi & 3) >> 1);
 
     f32x16 s[NK / 32];
-    auto score = [&](int buffer) {
-      const unsigned char* kt = lds + buffer * 2 * kTileBytes;
+    auto score = [&](int shift) {
+      const unsigned char* kt = lds + shift;
 #pragma unroll
       for (int b = 0; b < NK / 32; ++b) s[b] = f32x16{};
 #pragma unroll
@@ -358,8 +356,8 @@ struct Core {
           total += s[b][i];
         }
     };
-    auto collect = [&](int buffer) {
-      const unsigned char* vt = lds + buffer * 2 * kTileBytes + kTileBytes;
+    auto collect = [&](int shift) {
+      const unsigned char* vt = lds + shift + kTileBytes;
 #pragma unroll
       for (int step = 0; step < NK / 16; ++step) {
         // The B operand of 16 keys: a lane's eight weights as they are; the
@@ -391,113 +389,123 @@ struct Core {
 
     if constexpr (WR == 1) {
       // The next keys are on their way from the moment these are read, the next
-      // values likewise: one buffer, and no wave waits for another.
-      wait_loads();
-      for (int key = wave_begin; key < wave_end; key += TR) {
-        const bool more = key + TR < wave_end;
-        wait_loads_but<ValueLoader::kLoads>();
-        score(0);
-        wait_reads();
-        if (more) load_keys(0, key + TR);
-        weigh(key);
-        if (more) wait_loads_but<KeyLoader::kLoads>();
-        else wait_loads_but<0>();
-        collect(0);
-        wait_reads();
-        if (more) load_values(0, key + TR);
+      // values likewise: one buffer, and no wave waits for another. The pass
+      // before the first key only loads.
+      for (int key = wave_begin - TR; key < wave_end; key += TR) {
+        const bool here = key >= wave_begin, more = key + TR < wave_end;
+        if (here) {
+          wait_loads_but<ValueLoader::kLoads>();
+          score(0);
+          wait_reads();
+        }
+        if (more) key_loader.load(t.k, t.k_row, key + TR, last, 0, size);
+        if (here) {
+          weigh(key);
+          if (more) wait_loads_but<KeyLoader::kLoads>();
+          else wait_loads_but<0>();
+          collect(0);
+          wait_reads();
+        }
+        if (more) value_loader.load(t.v, t.v_row, key + TR, last, 0, size);
+        if (!here) wait_loads();  // the queries too
       }
     } else {
-      // One pass a buffer. The barrier: this buffer's tile is here, and the
-      // other one's readers are done.
-      auto pass = [&](int buffer, int key) {
+      // Two buffers. The barrier: this one's tile is here, and the other one's
+      // readers are done.
+      int shift = 0;
+      for (int key = t.begin - TR; key < end; key += TR) {
         wait_loads();
         __syncthreads();
+        shift ^= 2 * kTileBytes;
         if (key + TR < end) {
-          load_keys(buffer ^ 1, key + TR);
-          load_values(buffer ^ 1, key + TR);
+          key_loader.load(t.k, t.k_row, key + TR, last, shift, size);
+          value_loader.load(t.v, t.v_row, key + TR, last, shift, size);
         }
-        const int mine = key + wk * NK;
-        if (mine < wave_end) {
-          score(buffer);
+        const int mine = key + wk * NK, from = shift ^ 2 * kTileBytes;
+        if (key >= t.begin && mine < wave_end) {
+          score(from);
           weigh(mine);
-          collect(buffer);
+          collect(from);
         }
-      };
-      for (int key = t.begin; key < end; key += 2 * TR) {
-        pass(0, key);
-        if (key + TR < end) pass(1, key + TR);
       }
     }
     total += other_half(total);
 
-    // Sums, [wave][32 rows][D] with the 16-byte chunks of a row swizzled; then
-    // every row by half a wave.
-    __syncthreads();
-    float* sums = reinterpret_cast<float*>(lds) + wave * 32 * D;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int chunk = 8 * i + 2 * j + half;
-        *reinterpret_cast<f32x4*>(sums + col * D + ((chunk ^ (col & (D / 4 - 1))) << 2)) =
-            f32x4{acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]};
-      }
+    // The shares of a row agree on one reference; a wave scales its sums to it
+    // (to the finished row's scale where the row ends here) and leaves them in
+    // LDS, [wave][32 rows][D] with the 16-byte chunks of a row swizzled.
     if (half == 0) {
       marks[(wave * 32 + col) * 2] = ref - kLift;
       marks[(wave * 32 + col) * 2 + 1] = total;
     }
     const bool any_masked = __syncthreads_or(masked);
-    constexpr int kLanes = D / 4;  // lanes a row, four channels each
-    for (int r0 = wave * (64 / kLanes); r0 < t.rows; r0 += 4 * (64 / kLanes)) {
-      const int r = r0 + lane / kLanes, chunk = lane % kLanes;
-      float o[4] = {}, top = -kInf, sum = 0.0f;
-      if (r < t.rows) {
-        const int w0 = (r / 32) * WK, rc = r % 32;
+    float top = -kInf, sum = 0.0f, factor;
+    {
+      float m[WK];
 #pragma unroll
-        for (int w = 0; w < WK; ++w) top = fmaxf(top, marks[((w0 + w) * 32 + rc) * 2]);
-#pragma unroll
-        for (int w = 0; w < WK; ++w) {
-          const float m = marks[((w0 + w) * 32 + rc) * 2];
-          const float keep = m == -kInf ? 0.0f : m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-          sum += keep * marks[((w0 + w) * 32 + rc) * 2 + 1];
-          const f32x4 v = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds) + ((w0 + w) * 32 + rc) * D + ((chunk ^ (rc & (D / 4 - 1))) << 2));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] += m == -kInf && v[i] == v[i] ? 0.0f : keep * v[i];
-        }
+      for (int w = 0; w < WK; ++w) {
+        m[w] = marks[((wr * WK + w) * 32 + col) * 2];
+        top = fmaxf(top, m[w]);
       }
+      auto weight = [&](float x) { return x == -kInf ? 0.0f : x == top ? 1.0f : __builtin_amdgcn_exp2f(x - top); };
+#pragma unroll
+      for (int w = 0; w < WK; ++w) sum += weight(m[w]) * marks[((wr * WK + w) * 32 + col) * 2 + 1];
+      factor = weight(ref - kLift) * (sink.out ? sum == 0.0f ? 0.0f : 1.0f / sum : 1.0f);
+    }
+    if (half == 0 && wk == 0) {
+      marks[256 + my_row * 2] = top;
+      marks[256 + my_row * 2 + 1] = sum;
+    }
+    {
+      float* sums = reinterpret_cast<float*>(lds) + (wave * 32 + col) * D;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int chunk = 8 * i + 2 * j + half;
+          *reinterpret_cast<f32x4*>(sums + ((chunk ^ (col & (D / 4 - 1))) << 2)) =
+              f32x4{acc[i][4 * j] * factor, acc[i][4 * j + 1] * factor, acc[i][4 * j + 2] * factor, acc[i][4 * j + 3] * factor};
+        }
+    }
+    __syncthreads();
+    constexpr int kLanes = D / 4, kAt = 64 / kLanes;  // lanes a row, four channels each; rows a wave has at a time
+    const int chunk = lane % kLanes;
+    for (int r = wave * kAt + lane / kLanes; r - lane / kLanes < t.rows; r += 4 * kAt) {
+      const float* at = reinterpret_cast<const float*>(lds) + ((r / 32) * WK * 32 + r % 32) * D + ((chunk ^ (r % 32 & (D / 4 - 1))) << 2);
+      f32x4 o = *reinterpret_cast<const f32x4*>(at);
+#pragma unroll
+      for (int w = 1; w < WK; ++w) o += *reinterpret_cast<const f32x4*>(at + w * 32 * D);
+      const bool stored = r < t.rows && 4 * chunk < size;
+      f32x4 mark = {};
+      if (!sink.out) mark = f32x4{marks[256 + 2 * r], marks[256 + 2 * r + 1]};
       if (any_masked) {
-        const bool bad = r < t.rows && 4 * chunk < size && !(fabsf(o[0]) + fabsf(o[1]) + fabsf(o[2]) + fabsf(o[3]) < kInf);
-        unsigned long long rows_bad = __builtin_amdgcn_ballot_w64(bad);
-        for (int g = 0; g < 64 / kLanes; ++g) {
-          if (!(rows_bad >> (g * kLanes) & (kLanes == 64 ? ~0ull : (1ull << kLanes) - 1))) continue;
-          const int row = t.row0 + r0 + g;
-          const f32x4 v = slow_row(t.query(row), t.k, t.v, t.k_row, t.v_row, t.begin, t.limit(row), size, scale);
-          // Lane l holds channels 2 l, 2 l + 1.
-          float w[4];
-          for (int i = 0; i < 4; ++i) w[i] = __shfl(i & 1 ? v[1] : v[0], 2 * chunk + (i >> 1), 64);
-          if (lane / kLanes == g) {
-            for (int i = 0; i < 4; ++i) o[i] = w[i];
-            top = v[2];
-            sum = v[3];
+        const unsigned long long bad =
+            __builtin_amdgcn_ballot_w64(stored && !(fabsf(o[0]) + fabsf(o[1]) + fabsf(o[2]) + fabsf(o[3]) < kInf));
+        if (bad != 0) {
+          for (int g = 0; g < kAt; ++g) {
+            if (!(bad >> (g * kLanes) & (kLanes == 64 ? ~0ull : (1ull << kLanes) - 1))) continue;
+            const int row = r - lane / kLanes + g;
+            const f32x4 v = slow_row(t.query(row), t.k, t.v, t.k_row, t.v_row, t.begin, t.limit(row), size, scale);
+            // Lane l holds channels 2 l, 2 l + 1.
+            f32x4 w;
+            for (int i = 0; i < 4; ++i) w[i] = __shfl(i & 1 ? v[1] : v[0], 2 * chunk + (i >> 1), 64);
+            if (lane / kLanes == g) {
+              o = sink.out ? w * (v[3] == 0.0f ? 0.0f : 1.0f / v[3]) : w;
+              mark = f32x4{v[2], v[3]};
+            }
           }
         }
       }
-      if (r < t.rows && 4 * chunk < size) {
-        const int row = t.row0 + r;
-        if (sink.out) {
-          const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-          Q* dst = sink.out + (row / t.group) * sink.o_token + (row % t.group) * sink.o_head + 4 * chunk;
-          if constexpr (kSplit) {
-            *reinterpret_cast<f32x4*>(dst) = f32x4{o[0] * inverse, o[1] * inverse, o[2] * inverse, o[3] * inverse};
-          } else {
-            *reinterpret_cast<uint2*>(dst) = uint2{pack2<K>(o[0] * inverse, o[1] * inverse), pack2<K>(o[2] * inverse, o[3] * inverse)};
-          }
-        } else {
-          *reinterpret_cast<f32x4*>(sink.sums + (size_t)r * D + 4 * chunk) = f32x4{o[0], o[1], o[2], o[3]};
-          if (chunk == 0) {
-            sink.marks[2 * r] = top;
-            sink.marks[2 * r + 1] = sum;
-          }
+      if (!stored) continue;
+      if (sink.out) {
+        Q* dst = sink.out + t.token(r) * sink.o_token + t.head(r) * sink.o_head + 4 * chunk;
+        if constexpr (kSplit) *reinterpret_cast<f32x4*>(dst) = o;
+        else *reinterpret_cast<uint2*>(dst) = uint2{pack2<K>(o[0], o[1]), pack2<K>(o[2], o[3])};
+      } else {
+        *reinterpret_cast<f32x4*>(sink.sums + (size_t)r * D + 4 * chunk) = o;
+        if (chunk == 0) {
+          sink.marks[2 * r] = mark[0];
+          sink.marks[2 * r + 1] = mark[1];
         }
       }
     }
@@ -552,33 +560,35 @@ template <typename Q, typename K, int D, int WR, int WK, int NK>
 __global__ __launch_bounds__(kThreads) void packed_kernel(fah_packed_attention a, int slots, int splits) {
   using C = Core<Q, K, D, WR, WK, NK>;
   __shared__ __align__(16) unsigned char lds[C::kLds];
-  __shared__ float marks[256];
+  __shared__ float marks[512];
   const int group = a.heads / a.kv_heads, head = blockIdx.x % a.kv_heads;
   const int rest = blockIdx.x / a.kv_heads, split = rest % splits, slot = slots - 1 - rest / splits;
   const PackedTile p = packed_tile(a, slot, group, C::BM);
   if (p.rows == 0) return;
+  const int token0 = p.row0 / group;
   Task<Q, K> t;
-  t.q = static_cast<const Q*>(a.query) + p.begin * a.query_row + (int64_t)head * group * a.query_head;
+  t.q = static_cast<const Q*>(a.query) + (int64_t)(p.begin + token0) * a.query_row + (int64_t)head * group * a.query_head;
   t.q_token = a.query_row;
   t.q_head = a.query_head;
   t.k = static_cast<const K*>(a.key) + p.key_begin * a.key_row + head * a.key_head;
   t.v = static_cast<const K*>(a.value) + p.key_begin * a.value_row + head * a.value_head;
   t.k_row = (unsigned)a.key_row;
   t.v_row = (unsigned)a.value_row;
-  t.row0 = p.row0;
   t.rows = p.rows;
   t.group = group;
-  t.first_limit = p.first_limit;
+  t.group_inverse = 1.0f / (float)group;
+  t.head0 = p.row0 - token0 * group;
+  t.first_limit = p.first_limit + token0;
   t.causal = true;
   t.begin = 0;
   t.end = p.keys;
   Sink<Q> sink{};
   if (splits == 1) {
-    sink.out = static_cast<Q*>(a.output) + p.begin * a.output_row + (int64_t)head * group * a.output_head;
+    sink.out = static_cast<Q*>(a.output) + (int64_t)(p.begin + token0) * a.output_row + (int64_t)head * group * a.output_head;
     sink.o_token = a.output_row;
     sink.o_head = a.output_head;
   } else {
-    const int visible = clamp_int(t.limit(p.row0 + p.rows - 1), 0, p.keys);
+    const int visible = clamp_int(t.limit(p.rows - 1), 0, p.keys);
     const int share = ((visible + C::TR - 1) / C::TR + splits - 1) / splits * C::TR;
     t.begin = split * share;
     t.end = t.begin + share < visible ? t.begin + share : visible;
@@ -667,7 +677,7 @@ template <typename Q, typename K, int D, int WR, int WK, int NK>
 __global__ __launch_bounds__(kThreads) void prefix_kernel(fah_prefix_attention a, PrefixCut cut) {
   constexpr int kLds = std::max(Core<Q, K, D, WR, WK, NK>::kLds, Core<Q, K, D, 1, 4, 32>::kLds);
   __shared__ __align__(16) unsigned char lds[kLds];
-  __shared__ float marks[256];
+  __shared__ float marks[512];
   const int group = a.heads / a.kv_heads;
   float* partial = static_cast<float*>(a.workspace);
   Task<Q, K> t;
@@ -675,26 +685,28 @@ __global__ __launch_bounds__(kThreads) void prefix_kernel(fah_prefix_attention a
   t.q_token = a.query_sequence;
   t.q_head = a.query_head;
   t.group = group;
+  t.group_inverse = 1.0f / (float)group;
   t.causal = false;
   if (blockIdx.x < cut.prefix_items) {
     using C = Core<Q, K, D, WR, WK, NK>;
     const int head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
     const int share_at = rest % cut.shares, tile = rest / cut.shares;
     const int all = a.sequences * group;
-    t.q = static_cast<const Q*>(a.query) + (int64_t)head * group * a.query_head;
+    const int row0 = tile * C::BM, token0 = row0 / group;
+    t.head0 = row0 - token0 * group;
+    t.q = static_cast<const Q*>(a.query) + token0 * a.query_sequence + (int64_t)head * group * a.query_head;
     t.k = static_cast<const K*>(a.prefix_key) + head * a.prefix_key_head;
     t.v = static_cast<const K*>(a.prefix_value) + head * a.prefix_value_head;
     t.k_row = (unsigned)a.prefix_key_row;
     t.v_row = (unsigned)a.prefix_value_row;
-    t.row0 = tile * C::BM;
-    t.rows = clamp_int(all - t.row0, 0, C::BM);
+    t.rows = clamp_int(all - row0, 0, C::BM);
     const int share = ((a.prefix + C::TR - 1) / C::TR + cut.shares - 1) / cut.shares * C::TR;
     t.begin = share_at * share;
     t.end = t.begin + share < a.prefix ? t.begin + share : a.prefix;
     t.first_limit = t.end;
     const size_t rows = ((size_t)head * cut.shares + share_at) * all;
-    sink.sums = partial + rows * (D + 2) + (size_t)t.row0 * D;
-    sink.marks = partial + rows * (D + 2) + (size_t)all * D + 2 * t.row0;
+    sink.sums = partial + rows * (D + 2) + (size_t)row0 * D;
+    sink.marks = partial + rows * (D + 2) + (size_t)all * D + 2 * row0;
     C::run(t, sink, a.head_size, a.scale, lds, marks);
   } else {
     using C = Core<Q, K, D, 1, 4, 32>;
@@ -710,8 +722,8 @@ __global__ __launch_bounds__(kThreads) void prefix_kernel(fah_prefix_attention a
     t.v = static_cast<const K*>(a.value) + s * a.value_sequence + head * a.value_head;
     t.k_row = (unsigned)a.key_row;
     t.v_row = (unsigned)a.value_row;
-    t.row0 = tile * C::BM;
-    t.rows = clamp_int(group - t.row0, 0, C::BM);
+    t.head0 = tile * C::BM;
+    t.rows = clamp_int(group - t.head0, 0, C::BM);
     const int share = ((length + C::TR - 1) / C::TR + cut.own_shares - 1) / cut.own_shares * C::TR;
     t.begin = share_at * share;
     t.end = t.begin + share < length ? t.begin + share : length;
@@ -723,8 +735,8 @@ __global__ __launch_bounds__(kThreads) void prefix_kernel(fah_prefix_attention a
     } else {
       const size_t rows = (size_t)a.kv_heads * cut.shares * a.sequences * group * (cut.prefix_items ? 1 : 0) +
                           (((size_t)s * a.kv_heads + head) * cut.own_shares + share_at) * group;
-      sink.sums = partial + rows * (D + 2) + (size_t)t.row0 * D;
-      sink.marks = partial + rows * (D + 2) + (size_t)group * D + 2 * t.row0;
+      sink.sums = partial + rows * (D + 2) + (size_t)t.head0 * D;
+      sink.marks = partial + rows * (D + 2) + (size_t)group * D + 2 * t.head0;
     }
     C::run(t, sink, a.head_size, a.scale, lds, marks);
   }
