@@ -60,6 +60,11 @@ struct Task {
   int begin, end;            // keys
   int first_limit;           // token 0 sees the keys below this; per token one more if causal
   bool causal;
+  // A second range, the keys [0, more_end) of other rows, which every token
+  // sees (one group of rows only; 0: none).
+  const K *more_k, *more_v;
+  unsigned more_k_row, more_v_row;
+  int more_end;
   // Row r's token and head. (r + head0 is below 2^20: the product is within a
   // quarter of the exact quotient, which is at least half a step from a whole
   // number's edge.)
@@ -94,15 +99,22 @@ struct Tile {
   __device__ static int value_swizzle(int r) { return D == 128 ? (r & 3) << 2 : (r & 2) << 1; }
 };
 
+// A value that all lanes share, in scalar registers.
+__device__ __forceinline__ unsigned uniform(unsigned v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ const void* uniform(const void* p) {
+  const uint64_t v = (uint64_t)p;
+  return (const void*)((uint64_t)uniform((unsigned)(v >> 32)) << 32 | uniform((unsigned)v));
+}
+
 // 16 bytes a lane from base + offset to LDS at `to` + 16 lane. Inline, because
 // the compiler would wait for a load into LDS before any read of LDS: the
 // tiles' reads are ordered by wait_loads and a barrier instead. (It has no
 // register that it writes; a load into M0's place needs one wait state.)
 __device__ __forceinline__ void load_lds(const void* base, unsigned offset, unsigned to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(uniform(to)), "v"(offset), "s"(uniform(base)) : "memory");
 }
 __device__ __forceinline__ void load_lds(const void* from, unsigned to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(uniform(to)), "v"(from) : "memory");
 }
 // Every load of this wave is done (vmcnt 0, nothing else waited for). A barrier
 // follows: reads of LDS may move up to it but not before it.
@@ -170,18 +182,21 @@ struct Loader {
 // read: for rows whose tile held infinities or NaN where they are masked.
 // The lane's two sums, then the row's reference and total.
 template <typename Q, typename K>
-__device__ __noinline__ f32x4 slow_row(const Q* q, const K* k, const K* v_rows, unsigned k_row, unsigned v_row, int begin,
-                                       int lim, int size, float scale) {
-  const int lane = threadIdx.x & 63;
+__device__ __noinline__ f32x4 slow_row(const Q* q, const K* k_rows, const K* v_rows, unsigned k_row, unsigned v_row, int begin,
+                                       int lim, const K* more_k, const K* more_v, unsigned more_k_row, unsigned more_v_row,
+                                       int more_end, int size, float scale) {
+  const int lane = threadIdx.x & 63, count = lim > begin ? lim - begin : 0;
   float x[2] = {}, sum[2] = {}, top = -kInf, total = 0.0f;
   for (int i = 0; i < 2; ++i)
     if (2 * lane + i < size) x[i] = (float)q[2 * lane + i];
-  for (int key = begin; key < lim; ++key) {
+  for (int n = 0; n < count + more_end; ++n) {
+    const K* k = n < count ? k_rows + (int64_t)(begin + n) * k_row : more_k + (int64_t)(n - count) * more_k_row;
+    const K* w = n < count ? v_rows + (int64_t)(begin + n) * v_row : more_v + (int64_t)(n - count) * more_v_row;
     float s = 0.0f, v[2] = {};
     for (int i = 0; i < 2; ++i)
       if (2 * lane + i < size) {
-        s += x[i] * (float)k[(int64_t)key * k_row + 2 * lane + i];
-        v[i] = (float)v_rows[(int64_t)key * v_row + 2 * lane + i];
+        s += x[i] * (float)k[2 * lane + i];
+        v[i] = (float)w[2 * lane + i];
       }
     for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
     s *= scale * kLog2e;
@@ -207,41 +222,40 @@ __device__ __forceinline__ unsigned pack2(float a, float b) {
   }
 }
 
-// The workgroup's four waves as WR groups of 32 rows times WK shares of each
-// key tile; a wave takes NK keys of a tile.
+// The workgroup's waves as WR groups of 32 rows times WK shares of each key
+// tile; a wave takes NK keys of a tile.
 template <typename Q, typename K, int D, int WR, int WK, int NK>
 struct Core {
-  static constexpr int BM = 32 * WR, TR = WK * NK;
+  static constexpr int kWaves = WR * WK, kThreads = 64 * kWaves, BM = 32 * WR, TR = WK * NK;
   static constexpr int kTileBytes = TR * 2 * D;        // keys, or values
   // One group of rows: each wave's keys and values are its own, in one buffer.
   // Several groups share them, in two.
-  static constexpr int kBuffers = WR == 1 ? 1 : 2, kLds = kBuffers * 2 * kTileBytes;
+  static constexpr int kTiles = (WR == 1 ? 2 : 4) * kTileBytes, kSums = WK == 1 ? 0 : kWaves * 32 * D * 4;
+  static constexpr int kLds = kTiles > kSums ? kTiles : kSums, kMarks = 2 * 32 * (kWaves + WR);
   static constexpr bool kSplit = std::is_same_v<Q, float>;
   static constexpr int kSteps = D / 16;
 
-  // lds: two buffers of a key tile and a value tile; at the end the waves'
-  // sums. marks: [4][32][2], then
-  // [128][2].
+  // lds: one or two buffers of a key tile and a value tile; at the end the
+  // waves' sums. marks: [kWaves][32][2] of the waves, then [BM][2] of the rows.
   __device__ static void run(const Task<Q, K>& t, const Sink<Q>& sink, int size, float scale, unsigned char* lds,
                              float* marks) {
-    static_assert(kLds >= 4 * 32 * D * 4);
     using T = Tile<D>;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
     const int wr = wave / WK, wk = wave % WK;
     const int my_row = wr * 32 + col;
     const bool valid = my_row < t.rows;
-    const int lim = valid ? t.limit(my_row) : 0;
+    int lim = valid ? t.limit(my_row) : 0;
     const int wave_rows = clamp_int(t.rows - wr * 32, 0, 32);
-    const int lim_low = wave_rows ? t.limit(wr * 32) : 0;
-    const int lim_high = wave_rows ? t.limit(wr * 32 + wave_rows - 1) : 0;
-    const int end = t.limit(t.rows - 1);  // of the workgroup
+    int lim_low = wave_rows ? (int)uniform(t.limit(wr * 32)) : 0;
+    const int lim_high = wave_rows ? (int)uniform(t.limit(wr * 32 + wave_rows - 1)) : 0;
+    const int end = (int)uniform(t.limit(t.rows - 1));  // of the workgroup
     const int last = t.end - 1;
 
     if (D != size) {
-      for (int i = tid; i < kLds / 16; i += kThreads) reinterpret_cast<uint4*>(lds)[i] = uint4{0, 0, 0, 0};
+      for (int i = tid; i < kTiles / 16; i += kThreads) reinterpret_cast<uint4*>(lds)[i] = uint4{0, 0, 0, 0};
       __syncthreads();
     }
-    constexpr int kOwn = WR == 1 ? NK : TR, kLoaders = WR == 1 ? 1 : 4;
+    constexpr int kOwn = WR == 1 ? NK : TR, kLoaders = WR == 1 ? 1 : kWaves;
     const int own = WR == 1 ? wave * NK : 0, loader = WR == 1 ? 0 : wave;
     using KeyLoader = Loader<K, D, kOwn, kLoaders, false>;
     using ValueLoader = Loader<K, D, kOwn, kLoaders, true>;
@@ -250,49 +264,63 @@ struct Core {
     // The wave's first key, and the end of those that its rows see.
     const int wave_begin = t.begin + wk * NK, wave_end = lim_high;
 
-    // Queries: the B operand, lane (row col, channels 16 s + 8 half ..). fp32
-    // queries are scaled by a power of two to below 2^14 and split into two
+    // Queries: the B operand, lane (row col, channels 16 s + 8 half ..). They
+    // are requested here and looked at once the first tile is requested too.
+    // fp32 queries are scaled by a power of two to below 2^14 and split into two
     // fp16 parts (22 bits; the scale keeps the second part normal).
     s16x8 qf[kSplit ? 2 : 1][kSteps];
+    f32x4 raw[kSplit ? kSteps : 1][2];
     float c = scale * kLog2e;
     {
       const Q* q = t.query(valid ? my_row : 0);
-      if constexpr (kSplit) {
-        f32x4 x[kSteps][2];
-        float most = 0.0f;
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int d = 16 * s + 8 * half + 4 * i;
-            x[s][i] = valid && d < size ? *reinterpret_cast<const f32x4*>(q + d) : f32x4{};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(x[s][i][j]));
-          }
-        most = fmaxf(most, other_half(most));
-        const int e = (int)(f2u(most) >> 23) - 127;
-        const int up = e == 128 ? 0 : clamp_int(13 - e, -114, 126);
-        const float lift = u2f((unsigned)(up + 127) << 23);
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          f16x8 hi, lo;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float v = x[s][j >> 2][j & 3] * lift;
-            hi[j] = (_Float16)v;
-            lo[j] = (_Float16)(v - (float)hi[j]);
-          }
-          qf[0][s] = __builtin_bit_cast(s16x8, hi);
-          qf[kSplit ? 1 : 0][s] = __builtin_bit_cast(s16x8, lo);
-        }
-        c = fmaxf(c * u2f((unsigned)(127 - up) << 23), 1.2e-38f);
-      } else {
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          const int d = 16 * s + 8 * half;
-          qf[0][s] = valid && d < size ? *reinterpret_cast<const s16x8*>(q + d) : s16x8{};
+      for (int s = 0; s < kSteps; ++s) {
+        // (Channels behind head_size are asked for at 0, and cleared below.)
+        const int d = 16 * s + 8 * half < size ? 16 * s + 8 * half : 0;
+        if constexpr (kSplit) {
+          raw[s][0] = *reinterpret_cast<const f32x4*>(q + d);
+          raw[s][1] = *reinterpret_cast<const f32x4*>(q + d + 4);
+        } else {
+          qf[0][s] = *reinterpret_cast<const s16x8*>(q + d);
         }
       }
+    }
+    if (WR == 1 ? wave_begin < wave_end : t.begin < end) {
+      key_loader.load(t.k, t.k_row, t.begin + own, last, 0, size);
+      value_loader.load(t.v, t.v_row, t.begin + own, last, 0, size);
+    }
+    wait_loads();  // of the queries, as the compiler must know
+    if (D != size) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        if (16 * s + 8 * half >= size) {
+          if constexpr (kSplit) raw[s][0] = raw[s][1] = f32x4{};
+          else qf[0][s] = s16x8{};
+        }
+    }
+    if constexpr (kSplit) {
+      float most = 0.0f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(raw[s][j >> 2][j & 3]));
+      most = fmaxf(most, other_half(most));
+      const int e = (int)(f2u(most) >> 23) - 127;
+      const int up = e == 128 ? 0 : clamp_int(13 - e, -114, 126);
+      const float lift = u2f((unsigned)(up + 127) << 23);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        f16x8 hi, lo;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float v = raw[s][j >> 2][j & 3] * lift;
+          hi[j] = (_Float16)v;
+          lo[j] = (_Float16)(v - (float)hi[j]);
+        }
+        qf[0][s] = __builtin_bit_cast(s16x8, hi);
+        qf[kSplit ? 1 : 0][s] = __builtin_bit_cast(s16x8, lo);
+      }
+      c = fmaxf(c * u2f((unsigned)(127 - up) << 23), 1.2e-38f);
     }
 
     f32x16 acc[D / 32];
@@ -389,48 +417,123 @@ struct Core {
 
     if constexpr (WR == 1) {
       // The next keys are on their way from the moment these are read, the next
-      // values likewise: one buffer, and no wave waits for another. The pass
-      // before the first key only loads.
-      for (int key = wave_begin - TR; key < wave_end; key += TR) {
-        const bool here = key >= wave_begin, more = key + TR < wave_end;
-        if (here) {
+      // values likewise: one buffer, and no wave waits for another.
+      const K *k = t.k, *v = t.v;
+      unsigned k_row = t.k_row, v_row = t.v_row;
+      int from = wave_begin, to = wave_end, at_most = last;
+      KeyLoader keys = key_loader;
+      ValueLoader values = value_loader;
+      for (bool more_rows = t.more_end > 0;; more_rows = false) {
+        for (int key = from; key < to; key += TR) {
+          const bool more = key + TR < to;
           wait_loads_but<ValueLoader::kLoads>();
           score(0);
           wait_reads();
-        }
-        if (more) key_loader.load(t.k, t.k_row, key + TR, last, 0, size);
-        if (here) {
+          if (more) keys.load(k, k_row, key + TR, at_most, 0, size);
           weigh(key);
           if (more) wait_loads_but<KeyLoader::kLoads>();
           else wait_loads_but<0>();
           collect(0);
           wait_reads();
+          if (more) values.load(v, v_row, key + TR, at_most, 0, size);
         }
-        if (more) value_loader.load(t.v, t.v_row, key + TR, last, 0, size);
-        if (!here) wait_loads();  // the queries too
+        if (!more_rows) break;
+        k = t.more_k;
+        v = t.more_v;
+        k_row = t.more_k_row;
+        v_row = t.more_v_row;
+        from = wk * NK;
+        to = lim_low = t.more_end;
+        lim = valid ? t.more_end : 0;
+        at_most = t.more_end - 1;
+        keys = KeyLoader(lds + own * T::kRowBytes, k_row, loader);
+        values = ValueLoader(lds + kTileBytes + own * T::kRowBytes, v_row, loader);
+        if (from < to) {
+          keys.load(k, k_row, from, at_most, 0, size);
+          values.load(v, v_row, from, at_most, 0, size);
+        }
       }
     } else {
       // Two buffers. The barrier: this one's tile is here, and the other one's
       // readers are done.
       int shift = 0;
-      for (int key = t.begin - TR; key < end; key += TR) {
+      for (int key = t.begin; key < end; key += TR) {
         wait_loads();
         __syncthreads();
+        const int from = shift;
         shift ^= 2 * kTileBytes;
         if (key + TR < end) {
           key_loader.load(t.k, t.k_row, key + TR, last, shift, size);
           value_loader.load(t.v, t.v_row, key + TR, last, shift, size);
         }
-        const int mine = key + wk * NK, from = shift ^ 2 * kTileBytes;
-        if (key >= t.begin && mine < wave_end) {
+        if (key + wk * NK < wave_end) {
           score(from);
-          weigh(mine);
+          weigh(key + wk * NK);
           collect(from);
         }
       }
     }
     total += other_half(total);
 
+    if constexpr (WK == 1) {
+      // The rows are the wave's own: from registers to memory, a lane four
+      // channels of eight, both halves together 16 or 32 bytes.
+      const float top = ref == -kInf ? ref : ref - kLift;
+      const float factor = !sink.out ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
+      bool bad = false;
+      if (masked) {
+        float most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (D == size || 32 * i + 8 * (j >> 2) + 4 * half < size) most += fabsf(acc[i][j]);
+        bad = valid && !(most + other_half(most) < kInf);
+      }
+      if (valid && !bad) {
+        if (sink.out) {
+          Q* dst = sink.out + t.token(my_row) * sink.o_token + t.head(my_row) * sink.o_head + 4 * half;
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int d = 32 * i + 8 * j;
+              if (D != size && d + 4 * half >= size) continue;
+              const f32x4 o = f32x4{acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]} * factor;
+              if constexpr (kSplit) *reinterpret_cast<f32x4*>(dst + d) = o;
+              else *reinterpret_cast<uint2*>(dst + d) = uint2{pack2<K>(o[0], o[1]), pack2<K>(o[2], o[3])};
+            }
+        } else {
+          float* dst = sink.sums + (size_t)my_row * D + 4 * half;
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<f32x4*>(dst + 32 * i + 8 * j) =
+                  f32x4{acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]};
+          if (half == 0) {
+            sink.marks[2 * my_row] = top;
+            sink.marks[2 * my_row + 1] = total;
+          }
+        }
+      }
+      for (unsigned rows_bad = (unsigned)__builtin_amdgcn_ballot_w64(bad); rows_bad != 0; rows_bad &= rows_bad - 1) {
+        const int r = wr * 32 + __builtin_ctz(rows_bad);
+        const f32x4 v = slow_row(t.query(r), t.k, t.v, t.k_row, t.v_row, t.begin, t.limit(r), t.more_k, t.more_v, t.more_k_row,
+                                 t.more_v_row, t.more_end, size, scale);
+        for (int i = 0; i < 2; ++i) {
+          const int d = 2 * lane + i;
+          if (d >= size) continue;
+          if (sink.out) sink.out[t.token(r) * sink.o_token + t.head(r) * sink.o_head + d] = (Q)(v[3] == 0.0f ? 0.0f : v[i] / v[3]);
+          else sink.sums[(size_t)r * D + d] = v[i];
+        }
+        if (!sink.out && lane == 0) {
+          sink.marks[2 * r] = v[2];
+          sink.marks[2 * r + 1] = v[3];
+        }
+      }
+      return;
+    }
     // The shares of a row agree on one reference; a wave scales its sums to it
     // (to the finished row's scale where the row ends here) and leaves them in
     // LDS, [wave][32 rows][D] with the 16-byte chunks of a row swizzled.
@@ -453,10 +556,10 @@ struct Core {
       factor = weight(ref - kLift) * (sink.out ? sum == 0.0f ? 0.0f : 1.0f / sum : 1.0f);
     }
     if (half == 0 && wk == 0) {
-      marks[256 + my_row * 2] = top;
-      marks[256 + my_row * 2 + 1] = sum;
+      marks[64 * kWaves + my_row * 2] = top;
+      marks[64 * kWaves + my_row * 2 + 1] = sum;
     }
-    {
+    if (valid) {
       float* sums = reinterpret_cast<float*>(lds) + (wave * 32 + col) * D;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
@@ -470,14 +573,14 @@ struct Core {
     __syncthreads();
     constexpr int kLanes = D / 4, kAt = 64 / kLanes;  // lanes a row, four channels each; rows a wave has at a time
     const int chunk = lane % kLanes;
-    for (int r = wave * kAt + lane / kLanes; r - lane / kLanes < t.rows; r += 4 * kAt) {
+    for (int r = wave * kAt + lane / kLanes; r - lane / kLanes < t.rows; r += kWaves * kAt) {
       const float* at = reinterpret_cast<const float*>(lds) + ((r / 32) * WK * 32 + r % 32) * D + ((chunk ^ (r % 32 & (D / 4 - 1))) << 2);
       f32x4 o = *reinterpret_cast<const f32x4*>(at);
 #pragma unroll
       for (int w = 1; w < WK; ++w) o += *reinterpret_cast<const f32x4*>(at + w * 32 * D);
       const bool stored = r < t.rows && 4 * chunk < size;
       f32x4 mark = {};
-      if (!sink.out) mark = f32x4{marks[256 + 2 * r], marks[256 + 2 * r + 1]};
+      if (!sink.out) mark = f32x4{marks[64 * kWaves + 2 * r], marks[64 * kWaves + 2 * r + 1]};
       if (any_masked) {
         const unsigned long long bad =
             __builtin_amdgcn_ballot_w64(stored && !(fabsf(o[0]) + fabsf(o[1]) + fabsf(o[2]) + fabsf(o[3]) < kInf));
@@ -485,7 +588,8 @@ struct Core {
           for (int g = 0; g < kAt; ++g) {
             if (!(bad >> (g * kLanes) & (kLanes == 64 ? ~0ull : (1ull << kLanes) - 1))) continue;
             const int row = r - lane / kLanes + g;
-            const f32x4 v = slow_row(t.query(row), t.k, t.v, t.k_row, t.v_row, t.begin, t.limit(row), size, scale);
+            const f32x4 v = slow_row(t.query(row), t.k, t.v, t.k_row, t.v_row, t.begin, t.limit(row), t.more_k, t.more_v,
+                                     t.more_k_row, t.more_v_row, t.more_end, size, scale);
             // Lane l holds channels 2 l, 2 l + 1.
             f32x4 w;
             for (int i = 0; i < 4; ++i) w[i] = __shfl(i & 1 ? v[1] : v[0], 2 * chunk + (i >> 1), 64);
@@ -514,42 +618,41 @@ struct Core {
 
 // ---- Packed prompts ---------------------------------------------------------------
 
-// The place of sequence s's first tile of BM rows among all tiles: sequences
-// may leave one tile each empty, so no sum over the earlier ones is needed.
-__device__ __forceinline__ int first_tile(const fah_packed_attention& a, int s, int group, int BM) {
-  return clamp_int(a.query_offsets[s], 0, a.query_rows) * group / BM + s;
-}
+// The place of a sequence's first tile of BM rows among all tiles: floor(first
+// row / BM) + its number. Sequences may so leave one tile each empty, and no sum
+// over the earlier ones is needed.
+struct PackedTile {
+  int begin, row0, rows, key_begin, keys, first_limit;  // rows 0: none
+};
 
-// The sequence whose tile `slot` is, or -1: 64 probes at a time.
-__device__ __forceinline__ int find_sequence(const fah_packed_attention& a, int slot, int group, int BM) {
+// A wave finds the tile's sequence with 64 probes at a time; the last ones read
+// all that the tile needs, so that up to 64 sequences cost one round of loads.
+__device__ __forceinline__ PackedTile packed_tile(const fah_packed_attention& a, int slot, int group, int BM) {
   const int lane = threadIdx.x & 63;
+  const int* ko = a.key_offsets ? a.key_offsets : a.query_offsets;
+  auto rows_at = [&](int s) { return clamp_int(a.query_offsets[s], 0, a.query_rows); };
+  PackedTile p{};
   int lo = 0, hi = a.sequences;
-  while (hi - lo > 1) {
+  while (hi - lo > 64) {
     const int step = (hi - lo + 63) / 64, probe = lo + lane * step;
-    const bool ok = probe < hi && first_tile(a, probe, group, BM) <= slot;
+    const bool ok = probe < hi && rows_at(probe) * group / BM + probe <= slot;
     const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(ok));
-    if (n == 0) return -1;
+    if (n == 0) return p;
     lo += (n - 1) * step;
     hi = lo + step < hi ? lo + step : hi;
   }
-  return first_tile(a, lo, group, BM) <= slot ? lo : -1;
-}
-
-struct PackedTile {
-  int sequence, begin, row0, rows, key_begin, keys, first_limit;  // rows 0: none
-};
-
-__device__ __forceinline__ PackedTile packed_tile(const fah_packed_attention& a, int slot, int group, int BM) {
-  PackedTile p{};
-  p.sequence = __builtin_amdgcn_readfirstlane(find_sequence(a, slot, group, BM));
-  if (p.sequence < 0) return p;
-  const int* ko = a.key_offsets ? a.key_offsets : a.query_offsets;
-  p.begin = clamp_int(a.query_offsets[p.sequence], 0, a.query_rows);
-  const int queries = clamp_int(a.query_offsets[p.sequence + 1], p.begin, a.query_rows) - p.begin;
-  p.key_begin = clamp_int(ko[p.sequence], 0, a.key_rows);
-  p.keys = clamp_int(ko[p.sequence + 1], p.key_begin, a.key_rows) - p.key_begin;
+  const int s = lo + lane < hi ? lo + lane : hi - 1;
+  const int q0 = rows_at(s), q1 = rows_at(s + 1), k0 = clamp_int(ko[s], 0, a.key_rows), k1 = clamp_int(ko[s + 1], 0, a.key_rows);
+  const int tile = q0 * group / BM + s;
+  const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lo + lane < hi && tile <= slot));
+  if (n == 0) return p;
+  auto of = [&](int v) { return __builtin_amdgcn_readlane(v, n - 1); };
+  p.begin = of(q0);
+  const int queries = of(q1) > p.begin ? of(q1) - p.begin : 0;
+  p.key_begin = of(k0);
+  p.keys = of(k1) > p.key_begin ? of(k1) - p.key_begin : 0;
   p.first_limit = p.keys - queries + 1;
-  p.row0 = (slot - first_tile(a, p.sequence, group, BM)) * BM;
+  p.row0 = (slot - of(tile)) * BM;
   p.rows = clamp_int(queries * group - p.row0, 0, BM);
   return p;
 }
@@ -557,10 +660,10 @@ __device__ __forceinline__ PackedTile packed_tile(const fah_packed_attention& a,
 // Workgroup: (tile from the last one on, share of the keys, K/V head), the K/V
 // head fastest, so that with 8 of them each XCD's L2 serves one head.
 template <typename Q, typename K, int D, int WR, int WK, int NK>
-__global__ __launch_bounds__(kThreads) void packed_kernel(fah_packed_attention a, int slots, int splits) {
+__global__ __launch_bounds__(64 * WR * WK, 2) void packed_kernel(fah_packed_attention a, int slots, int splits) {
   using C = Core<Q, K, D, WR, WK, NK>;
   __shared__ __align__(16) unsigned char lds[C::kLds];
-  __shared__ float marks[512];
+  __shared__ float marks[C::kMarks];
   const int group = a.heads / a.kv_heads, head = blockIdx.x % a.kv_heads;
   const int rest = blockIdx.x / a.kv_heads, split = rest % splits, slot = slots - 1 - rest / splits;
   const PackedTile p = packed_tile(a, slot, group, C::BM);
@@ -580,6 +683,7 @@ __global__ __launch_bounds__(kThreads) void packed_kernel(fah_packed_attention a
   t.head0 = p.row0 - token0 * group;
   t.first_limit = p.first_limit + token0;
   t.causal = true;
+  t.more_end = 0;
   t.begin = 0;
   t.end = p.keys;
   Sink<Q> sink{};
@@ -599,37 +703,44 @@ __global__ __launch_bounds__(kThreads) void packed_kernel(fah_packed_attention a
   C::run(t, sink, a.head_size, a.scale, lds, marks);
 }
 
-// Joins partial rows by groups of D / 4 lanes, four channels a lane: `count`
-// partial sums, sums at s0 + i * step and marks at m0 + i * step. The marks are
-// read by a lane each and shared, so that every load stands alone.
+// Joins partial rows by groups of D / 4 lanes, four channels a lane: at(i) is
+// where partial i's row has its sums, marks(i) its marks. The marks are read by
+// a lane each and shared, so that every load stands alone.
 template <int D>
 struct Joined {
   static constexpr int kLanes = D / 4;
   float top = -kInf, total = 0.0f;
   f32x4 o = {};
-  __device__ __forceinline__ void add(const float* sums, const float* marks, size_t step, int count) {
+  template <typename At, typename Marks>
+  __device__ __forceinline__ void add(int count, At at, Marks marks) {
     const int lane = threadIdx.x % kLanes;
     for (int first = 0; first < count; first += kLanes) {
       const int n = count - first < kLanes ? count - first : kLanes;
       float m = -kInf, w = 0.0f;
       if (lane < n) {
-        m = marks[(first + lane) * step];
-        w = marks[(first + lane) * step + 1];
+        const float2 mark = *reinterpret_cast<const float2*>(marks(first + lane));
+        m = mark.x;
+        w = mark.y;
       }
       float next = fmaxf(top, m);
       for (int x = kLanes / 2; x >= 1; x >>= 1) next = fmaxf(next, __shfl_xor(next, x, kLanes));
       // A partial row that saw nothing counts as nothing, unless its total is NaN.
-      const float weight = m == next && m != -kInf ? 1.0f : m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - next);
+      const float weight = m == -kInf ? 0.0f : m == next ? 1.0f : __builtin_amdgcn_exp2f(m - next);
       const float keep = top == -kInf || top == next ? 1.0f : __builtin_amdgcn_exp2f(top - next);
       float sum = w == w ? weight * w : w;
       for (int x = kLanes / 2; x >= 1; x >>= 1) sum += __shfl_xor(sum, x, kLanes);
       total = total * keep + sum;
       o *= keep;
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) {
-        const float wi = __shfl(weight, i, kLanes);
-        const f32x4 v = *reinterpret_cast<const f32x4*>(sums + (first + i) * step);
-        o += wi == 0.0f ? f32x4{} : v * wi;
+      // Eight at a time, all requested before the first is used.
+      for (int i0 = 0; i0 < n; i0 += 8) {
+        f32x4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const f32x4*>(at(first + (i0 + i < n ? i0 + i : n - 1)));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float wi = __shfl(weight, (i0 + i) % kLanes, kLanes);  // 0 from n on
+          o += i0 + i >= n || wi == 0.0f ? f32x4{} : v[i] * wi;
+        }
       }
       top = next;
     }
@@ -655,7 +766,8 @@ __global__ __launch_bounds__(kThreads) void packed_join_kernel(fah_packed_attent
   Q* out = static_cast<Q*>(a.output) + p.begin * a.output_row + (int64_t)head * group * a.output_head;
   for (int r = threadIdx.x / kLanes; r < p.rows; r += kThreads / kLanes) {
     Joined<D> j;
-    j.add(sums + r * D + 4 * chunk, sums + BM * D + 2 * r, BM * (D + 2), splits);
+    j.add(splits, [&](int i) { return sums + (size_t)i * BM * (D + 2) + r * D + 4 * chunk; },
+          [&](int i) { return sums + (size_t)i * BM * (D + 2) + BM * D + 2 * r; });
     const int row = p.row0 + r;
     if (4 * chunk < a.head_size) j.write(out + (row / group) * a.output_row + (row % group) * a.output_head + 4 * chunk);
   }
@@ -666,18 +778,22 @@ __global__ __launch_bounds__(kThreads) void packed_join_kernel(fah_packed_attent
 // How prefix_kernel's work is cut: prefix tiles of BM rows (a row is a sequence
 // and a head of the group) times shares of the prefix, then for every sequence
 // tiles of 32 heads times shares of its own rows.
+// `both`: few rows and keys; a sequence's tiles attend the prefix themselves.
 struct PrefixCut {
   int tiles, shares, own_tiles, own_shares;
+  bool both;
   int64_t prefix_items, own_items;
 };
 
 // Partial rows: [K/V head][share][sequences * group][D + 2] of the prefix, then
 // [sequence][K/V head][own share][group][D + 2]; a row's sums, then its marks.
 template <typename Q, typename K, int D, int WR, int WK, int NK>
-__global__ __launch_bounds__(kThreads) void prefix_kernel(fah_prefix_attention a, PrefixCut cut) {
-  constexpr int kLds = std::max(Core<Q, K, D, WR, WK, NK>::kLds, Core<Q, K, D, 1, 4, 32>::kLds);
-  __shared__ __align__(16) unsigned char lds[kLds];
-  __shared__ float marks[512];
+__global__ __launch_bounds__(kThreads, 2) void prefix_kernel(fah_prefix_attention a, PrefixCut cut) {
+  using Shared = Core<Q, K, D, WR, WK, NK>;
+  using Own = Core<Q, K, D, 1, 4, 32>;
+  static_assert(Shared::kThreads == kThreads && Own::kThreads == kThreads);
+  __shared__ __align__(16) unsigned char lds[std::max(Shared::kLds, Own::kLds)];
+  __shared__ float marks[std::max(Shared::kMarks, Own::kMarks)];
   const int group = a.heads / a.kv_heads;
   float* partial = static_cast<float*>(a.workspace);
   Task<Q, K> t;
@@ -687,8 +803,9 @@ __global__ __launch_bounds__(kThreads) void prefix_kernel(fah_prefix_attention a
   t.group = group;
   t.group_inverse = 1.0f / (float)group;
   t.causal = false;
+  t.more_end = 0;
   if (blockIdx.x < cut.prefix_items) {
-    using C = Core<Q, K, D, WR, WK, NK>;
+    using C = Shared;
     const int head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
     const int share_at = rest % cut.shares, tile = rest / cut.shares;
     const int all = a.sequences * group;
@@ -709,7 +826,7 @@ __global__ __launch_bounds__(kThreads) void prefix_kernel(fah_prefix_attention a
     sink.marks = partial + rows * (D + 2) + (size_t)all * D + 2 * row0;
     C::run(t, sink, a.head_size, a.scale, lds, marks);
   } else {
-    using C = Core<Q, K, D, 1, 4, 32>;
+    using C = Own;
     const int64_t at = blockIdx.x - cut.prefix_items;
     const int head = at % a.kv_heads;
     int64_t rest = at / a.kv_heads;
@@ -724,9 +841,23 @@ __global__ __launch_bounds__(kThreads) void prefix_kernel(fah_prefix_attention a
     t.v_row = (unsigned)a.value_row;
     t.head0 = tile * C::BM;
     t.rows = clamp_int(group - t.head0, 0, C::BM);
-    const int share = ((length + C::TR - 1) / C::TR + cut.own_shares - 1) / cut.own_shares * C::TR;
-    t.begin = share_at * share;
-    t.end = t.begin + share < length ? t.begin + share : length;
+    if (cut.both) {
+      t.more_k = t.k;
+      t.more_v = t.v;
+      t.more_k_row = t.k_row;
+      t.more_v_row = t.v_row;
+      t.more_end = length;
+      t.k = static_cast<const K*>(a.prefix_key) + head * a.prefix_key_head;
+      t.v = static_cast<const K*>(a.prefix_value) + head * a.prefix_value_head;
+      t.k_row = (unsigned)a.prefix_key_row;
+      t.v_row = (unsigned)a.prefix_value_row;
+      t.begin = 0;
+      t.end = a.prefix;
+    } else {
+      const int share = ((length + C::TR - 1) / C::TR + cut.own_shares - 1) / cut.own_shares * C::TR;
+      t.begin = share_at * share;
+      t.end = t.begin + share < length ? t.begin + share : length;
+    }
     t.first_limit = t.end;
     if (cut.prefix_items == 0 && cut.own_shares == 1) {
       sink.out = static_cast<Q*>(a.output) + s * a.output_sequence + (int64_t)head * group * a.output_head;
@@ -750,18 +881,23 @@ __global__ __launch_bounds__(kThreads) void prefix_join_kernel(fah_prefix_attent
   const int chunk = threadIdx.x % kLanes;
   if (at >= (int64_t)a.sequences * a.heads) return;
   const int s = at / a.heads, q_head = at % a.heads, head = q_head / group, g = q_head % group;
-  const float* partial = static_cast<const float*>(a.workspace);
+  // The prefix's shares, then the own rows'.
+  const int shares = cut.prefix_items ? cut.shares : 0;
+  const size_t step = (size_t)all * (D + 2), own_step = (size_t)group * (D + 2);
+  const float* shared = static_cast<const float*>(a.workspace) + (size_t)head * shares * step;
+  const float* own = static_cast<const float*>(a.workspace) + (size_t)a.kv_heads * shares * step +
+                     ((size_t)s * a.kv_heads + head) * cut.own_shares * own_step;
+  const int row = s * group + g;
   Joined<D> j;
-  if (cut.prefix_items) {
-    const size_t step = (size_t)all * (D + 2);
-    const float* from = partial + (size_t)head * cut.shares * step;
-    const int row = s * group + g;
-    j.add(from + (size_t)row * D + 4 * chunk, from + (size_t)all * D + 2 * row, step, cut.shares);
-    partial += (size_t)a.kv_heads * cut.shares * step;
-  }
-  const size_t step = (size_t)group * (D + 2);
-  const float* from = partial + ((size_t)s * a.kv_heads + head) * cut.own_shares * step;
-  j.add(from + (size_t)g * D + 4 * chunk, from + (size_t)group * D + 2 * g, step, cut.own_shares);
+  j.add(shares + cut.own_shares,
+        [&](int i) {
+          return i < shares ? shared + i * step + (size_t)row * D + 4 * chunk
+                            : own + (i - shares) * own_step + (size_t)g * D + 4 * chunk;
+        },
+        [&](int i) {
+          return i < shares ? shared + i * step + (size_t)all * D + 2 * row
+                            : own + (i - shares) * own_step + (size_t)group * D + 2 * g;
+        });
   if (4 * chunk < a.head_size) j.write(static_cast<Q*>(a.output) + s * a.output_sequence + q_head * a.output_head + 4 * chunk);
 }
 
@@ -772,7 +908,7 @@ constexpr int kFill = 512;  // workgroups that fill the chip
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct PackedCut {
-  int waves_rows;  // WR
+  int rows;  // WR
   int splits;
   int64_t slots;
 };
@@ -780,28 +916,28 @@ struct PackedCut {
 PackedCut packed_cut(const fah_packed_attention& a) {
   const int group = a.heads / a.kv_heads;
   const int64_t rows = (int64_t)a.query_rows * group;
+  auto items = [&](int waves) { return ceil_div(rows, 32 * waves) * a.kv_heads; };
   PackedCut c;
-  c.waves_rows = (int64_t)a.longest_query * group <= 32 || ceil_div(rows, 64) * a.kv_heads < kFill / 2 ? 1
-                 : ceil_div(rows, 128) * a.kv_heads < kFill                                            ? 2
-                                                                                                       : 4;
-  const int BM = 32 * c.waves_rows;
-  c.slots = rows / BM + a.sequences;
-  const int64_t items = ceil_div(rows, BM) * a.kv_heads;
-  c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kFill / items, ceil_div(a.longest_key, 512)));
+  c.rows = (int64_t)a.longest_query * group <= 32 || items(2) < kFill / 2 ? 1 : items(4) < kFill ? 2 : 4;
+  c.slots = rows / (32 * c.rows) + a.sequences;
+  c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kFill / items(c.rows), ceil_div(a.longest_key, 512)));
   return c;
 }
 
 PrefixCut prefix_cut(const fah_prefix_attention& a, int* waves_rows) {
-  const int group = a.heads / a.kv_heads;
+  const int group = a.heads / a.kv_heads, longest = std::min(a.longest, a.capacity);
   const int64_t rows = (int64_t)a.sequences * group;
-  *waves_rows = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
   PrefixCut c{};
-  c.tiles = (int)ceil_div(rows, 32 * *waves_rows);
-  c.shares = (int)std::max<int64_t>(1, std::min<int64_t>(kFill / (c.tiles * a.kv_heads), ceil_div(a.prefix, 256)));
-  c.prefix_items = a.prefix ? (int64_t)c.tiles * a.kv_heads * c.shares : 0;
   c.own_tiles = (int)ceil_div(group, 32);
   const int64_t own = (int64_t)a.sequences * a.kv_heads * c.own_tiles;
-  c.own_shares = (int)std::max<int64_t>(1, std::min<int64_t>(kFill / own, ceil_div(std::min(a.longest, a.capacity), 256)));
+  *waves_rows = rows <= 32 ? 1 : ceil_div(rows, 64) * a.kv_heads < 1024 ? 2 : 4;
+  c.own_shares = (int)std::max<int64_t>(1, std::min<int64_t>(256 / own, ceil_div(longest, 256)));
+  c.both = own <= 256 && (int64_t)a.prefix + longest <= 1024;
+  if (c.both) c.own_shares = 1, *waves_rows = 1;
+  c.tiles = (int)ceil_div(rows, 32 * *waves_rows);
+  const int64_t fill = own * c.own_shares >= 1024 ? 128 : 256;
+  c.shares = (int)std::max<int64_t>(1, std::min<int64_t>(fill / (c.tiles * a.kv_heads), ceil_div(a.prefix, 256)));
+  c.prefix_items = a.prefix && !c.both ? (int64_t)c.tiles * a.kv_heads * c.shares : 0;
   c.own_items = own * c.own_shares;
   return c;
 }
@@ -812,7 +948,7 @@ template <typename Q, typename K, int D, int WR, int WK, int NK>
 hipError_t packed_launch(const fah_packed_attention& a, const PackedCut& c, hipStream_t s) {
   using C = Core<Q, K, D, WR, WK, NK>;
   auto kernel = packed_kernel<Q, K, D, WR, WK, NK>;
-  kernel<<<(unsigned)(c.slots * c.splits * a.kv_heads), kThreads, 0, s>>>(a, (int)c.slots, c.splits);
+  kernel<<<(unsigned)(c.slots * c.splits * a.kv_heads), C::kThreads, 0, s>>>(a, (int)c.slots, c.splits);
   if (c.splits > 1)
     packed_join_kernel<Q, D, C::BM><<<(unsigned)(c.slots * a.kv_heads), kThreads, 0, s>>>(a, c.splits);
   return hipGetLastError();
@@ -821,8 +957,8 @@ hipError_t packed_launch(const fah_packed_attention& a, const PackedCut& c, hipS
 template <typename Q, typename K, int D>
 hipError_t packed_typed(const fah_packed_attention& a, hipStream_t s) {
   const PackedCut c = packed_cut(a);
-  if (c.waves_rows == 1) return packed_launch<Q, K, D, 1, 4, 32>(a, c, s);
-  if (c.waves_rows == 2) return packed_launch<Q, K, D, 2, 2, 32>(a, c, s);
+  if (c.rows == 1) return packed_launch<Q, K, D, 1, 4, 32>(a, c, s);
+  if (c.rows == 2) return packed_launch<Q, K, D, 2, 2, 32>(a, c, s);
   return packed_launch<Q, K, D, 4, 1, 64>(a, c, s);
 }
 
@@ -855,7 +991,7 @@ bool attention_supported(int heads, int kv_heads, int head_size, int query_type,
 int64_t packed_attention_workspace(const fah_packed_attention& a) {
   if (a.sequences == 0 || a.query_rows == 0) return 0;
   const PackedCut c = packed_cut(a);
-  return c.splits == 1 ? 0 : c.slots * a.kv_heads * c.splits * 32 * c.waves_rows * (width_of(a.head_size) + 2) * 4;
+  return c.splits == 1 ? 0 : c.slots * a.kv_heads * c.splits * 32 * c.rows * (width_of(a.head_size) + 2) * 4;
 }
 
 int64_t prefix_attention_workspace(const fah_prefix_attention& a) {
