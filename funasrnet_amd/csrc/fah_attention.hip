@@ -657,15 +657,32 @@ __device__ __forceinline__ PackedTile packed_tile(const fah_packed_attention& a,
   return p;
 }
 
-// Workgroup: (tile from the last one on, share of the keys, K/V head), the K/V
-// head fastest, so that with 8 of them each XCD's L2 serves one head.
+// How packed_kernel's work is cut: tiles (slots) of 32 `rows` rows, whose keys
+// are cut into shares of about `share`, at most `splits`.
+struct PackedCut {
+  int rows, splits, share;
+  int64_t slots;
+};
+
+// Keys that some row of the tile sees, and the shares they are cut into.
+__device__ __forceinline__ int visible_keys(const PackedTile& p, int group) {
+  return clamp_int(p.first_limit + (p.row0 + p.rows - 1) / group, 0, p.keys);
+}
+__device__ __forceinline__ int shares_of(int visible, const PackedCut& cut) {
+  return clamp_int((visible + cut.share / 2) / cut.share, 1, cut.splits);
+}
+
+// Workgroup: (share of the keys, tile from the last one on, K/V head), the K/V
+// head fastest, so that with 8 of them each XCD's L2 serves one head, and the
+// shares slowest: most tiles have one, and those that only find that out come
+// last (in between they hold up the others' start: 750 rows 22.9 -> 35 us).
 template <typename Q, typename K, int D, int WR, int WK, int NK>
-__global__ __launch_bounds__(64 * WR * WK, 2) void packed_kernel(fah_packed_attention a, int slots, int splits) {
+__global__ __launch_bounds__(64 * WR * WK, 2) void packed_kernel(fah_packed_attention a, PackedCut cut) {
   using C = Core<Q, K, D, WR, WK, NK>;
   __shared__ __align__(16) unsigned char lds[C::kLds];
   __shared__ float marks[C::kMarks];
   const int group = a.heads / a.kv_heads, head = blockIdx.x % a.kv_heads;
-  const int rest = blockIdx.x / a.kv_heads, split = rest % splits, slot = slots - 1 - rest / splits;
+  const int rest = blockIdx.x / a.kv_heads, split = rest / (int)cut.slots, slot = (int)cut.slots - 1 - rest % (int)cut.slots;
   const PackedTile p = packed_tile(a, slot, group, C::BM);
   if (p.rows == 0) return;
   const int token0 = p.row0 / group;
@@ -687,16 +704,17 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void packed_kernel(fah_packed_atte
   t.begin = 0;
   t.end = p.keys;
   Sink<Q> sink{};
-  if (splits == 1) {
+  const int visible = visible_keys(p, group), shares = shares_of(visible, cut);
+  if (split >= shares) return;
+  if (shares == 1) {
     sink.out = static_cast<Q*>(a.output) + (int64_t)(p.begin + token0) * a.output_row + (int64_t)head * group * a.output_head;
     sink.o_token = a.output_row;
     sink.o_head = a.output_head;
   } else {
-    const int visible = clamp_int(t.limit(p.rows - 1), 0, p.keys);
-    const int share = ((visible + C::TR - 1) / C::TR + splits - 1) / splits * C::TR;
+    const int share = ((visible + C::TR - 1) / C::TR + shares - 1) / shares * C::TR;
     t.begin = split * share;
     t.end = t.begin + share < visible ? t.begin + share : visible;
-    const size_t item = ((size_t)slot * a.kv_heads + head) * splits + split;
+    const size_t item = ((size_t)slot * a.kv_heads + head) * cut.splits + split;
     sink.sums = static_cast<float*>(a.workspace) + item * C::BM * (D + 2);
     sink.marks = sink.sums + C::BM * D;
   }
@@ -756,21 +774,24 @@ struct Joined {
   }
 };
 
+// Workgroup: (tile, K/V head), as many rows of it as it has groups of lanes.
 template <typename Q, int D, int BM>
-__global__ __launch_bounds__(kThreads) void packed_join_kernel(fah_packed_attention a, int splits) {
+__global__ __launch_bounds__(kThreads) void packed_join_kernel(fah_packed_attention a, PackedCut cut) {
   const int group = a.heads / a.kv_heads, head = blockIdx.x % a.kv_heads, slot = blockIdx.x / a.kv_heads;
   const PackedTile p = packed_tile(a, slot, group, BM);
   constexpr int kLanes = D / 4;
-  const int chunk = threadIdx.x % kLanes;
-  const float* sums = static_cast<const float*>(a.workspace) + ((size_t)slot * a.kv_heads + head) * splits * BM * (D + 2);
-  Q* out = static_cast<Q*>(a.output) + p.begin * a.output_row + (int64_t)head * group * a.output_head;
-  for (int r = threadIdx.x / kLanes; r < p.rows; r += kThreads / kLanes) {
-    Joined<D> j;
-    j.add(splits, [&](int i) { return sums + (size_t)i * BM * (D + 2) + r * D + 4 * chunk; },
-          [&](int i) { return sums + (size_t)i * BM * (D + 2) + BM * D + 2 * r; });
-    const int row = p.row0 + r;
-    if (4 * chunk < a.head_size) j.write(out + (row / group) * a.output_row + (row % group) * a.output_head + 4 * chunk);
-  }
+  const int chunk = threadIdx.x % kLanes, r = blockIdx.y * (kThreads / kLanes) + threadIdx.x / kLanes;
+  if (r >= p.rows) return;
+  const int shares = shares_of(visible_keys(p, group), cut);
+  if (shares == 1) return;
+  const float* sums = static_cast<const float*>(a.workspace) + ((size_t)slot * a.kv_heads + head) * cut.splits * BM * (D + 2);
+  Joined<D> j;
+  j.add(shares, [&](int i) { return sums + (size_t)i * BM * (D + 2) + r * D + 4 * chunk; },
+        [&](int i) { return sums + (size_t)i * BM * (D + 2) + BM * D + 2 * r; });
+  const int row = p.row0 + r;
+  if (4 * chunk < a.head_size)
+    j.write(static_cast<Q*>(a.output) + (int64_t)(p.begin + row / group) * a.output_row +
+            (int64_t)(head * group + row % group) * a.output_head + 4 * chunk);
 }
 
 // ---- A shared prefix ----------------------------------------------------------------
@@ -907,20 +928,19 @@ constexpr int kFill = 512;  // workgroups that fill the chip
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-struct PackedCut {
-  int rows;  // WR
-  int splits;
-  int64_t slots;
-};
-
 PackedCut packed_cut(const fah_packed_attention& a) {
   const int group = a.heads / a.kv_heads;
-  const int64_t rows = (int64_t)a.query_rows * group;
-  auto items = [&](int waves) { return ceil_div(rows, 32 * waves) * a.kv_heads; };
+  const int64_t rows = (int64_t)a.query_rows * group, keys = a.key_rows / a.sequences, rows_each = rows / a.sequences;
+  auto items = [&](int waves) { return std::max<int64_t>(ceil_div(rows, 32 * waves), a.sequences) * a.kv_heads; };
   PackedCut c;
-  c.rows = (int64_t)a.longest_query * group <= 32 || items(2) < kFill / 2 ? 1 : items(4) < kFill ? 2 : 4;
+  const bool cached = (a.key_rows - a.query_rows) / a.sequences >= 1024;
+  if ((int64_t)a.longest_query * group <= 32) c.rows = 1;
+  else if (cached) c.rows = rows_each >= 192 && items(4) * keys / 1280 >= 256 ? 4 : rows_each > 32 ? 2 : 1;
+  else c.rows = items(2) < kFill / 2 ? 1 : items(4) < kFill ? 2 : 4;
   c.slots = rows / (32 * c.rows) + a.sequences;
-  c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kFill / items(c.rows), ceil_div(a.longest_key, 512)));
+  const int64_t n = items(c.rows);
+  c.share = (int)std::min<int64_t>(std::max<int64_t>(512, n * keys / kFill), 1280);
+  c.splits = cached ? (int)std::max<int64_t>(1, std::min<int64_t>(2048 / n, (a.longest_key + c.share / 2) / c.share)) : 1;
   return c;
 }
 
@@ -948,9 +968,11 @@ template <typename Q, typename K, int D, int WR, int WK, int NK>
 hipError_t packed_launch(const fah_packed_attention& a, const PackedCut& c, hipStream_t s) {
   using C = Core<Q, K, D, WR, WK, NK>;
   auto kernel = packed_kernel<Q, K, D, WR, WK, NK>;
-  kernel<<<(unsigned)(c.slots * c.splits * a.kv_heads), C::kThreads, 0, s>>>(a, (int)c.slots, c.splits);
-  if (c.splits > 1)
-    packed_join_kernel<Q, D, C::BM><<<(unsigned)(c.slots * a.kv_heads), kThreads, 0, s>>>(a, c.splits);
+  kernel<<<(unsigned)(c.slots * c.splits * a.kv_heads), C::kThreads, 0, s>>>(a, c);
+  if (c.splits > 1) {
+    const dim3 grid((unsigned)(c.slots * a.kv_heads), C::BM / (kThreads / (D / 4)));
+    packed_join_kernel<Q, D, C::BM><<<grid, kThreads, 0, s>>>(a, c);
+  }
   return hipGetLastError();
 }
 
