@@ -231,14 +231,18 @@ struct Core {
   // One group of rows: each wave's keys and values are its own, in one buffer.
   // Several groups share them, in two.
   static constexpr int kTiles = (WR == 1 ? 2 : 4) * kTileBytes, kSums = WK == 1 ? 0 : kWaves * 32 * D * 4;
-  static constexpr int kLds = kTiles > kSums ? kTiles : kSums, kMarks = 2 * 32 * (kWaves + WR);
+  static constexpr int kArea = kTiles > kSums ? kTiles : kSums;
+  // Behind the area: one group of rows shares its queries' fragments there, and
+  // at the end the waves' references and totals stand there.
   static constexpr bool kSplit = std::is_same_v<Q, float>;
-  static constexpr int kSteps = D / 16;
+  static constexpr int kSteps = D / 16, kShared = WR == 1 ? kSteps * 1024 * (kSplit ? 2 : 1) : 0, kMarks = 8 * 32 * (kWaves + WR) + 4 * kWaves;
+  static constexpr int kLds = kArea + (kShared > kMarks ? kShared : kMarks);
 
   // lds: one or two buffers of a key tile and a value tile; at the end the
-  // waves' sums. marks: [kWaves][32][2] of the waves, then [BM][2] of the rows.
-  __device__ static void run(const Task<Q, K>& t, const Sink<Q>& sink, int size, float scale, unsigned char* lds,
-                             float* marks) {
+  // waves' sums. Behind them marks: [kWaves][32][2] of the waves, then [BM][2]
+  // of the rows, then whether each wave masked scores.
+  __device__ static void run(const Task<Q, K>& t, const Sink<Q>& sink, int size, float scale, unsigned char* lds) {
+    float* marks = reinterpret_cast<float*>(lds + kArea);
     using T = Tile<D>;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
     const int wr = wave / WK, wk = wave % WK;
@@ -264,24 +268,30 @@ struct Core {
     // The wave's first key, and the end of those that its rows see.
     const int wave_begin = t.begin + wk * NK, wave_end = lim_high;
 
-    // Queries: the B operand, lane (row col, channels 16 s + 8 half ..). They
-    // are requested here and looked at once the first tile is requested too.
-    // fp32 queries are scaled by a power of two to below 2^14 and split into two
-    // fp16 parts (22 bits; the scale keeps the second part normal).
-    s16x8 qf[kSplit ? 2 : 1][kSteps];
-    f32x4 raw[kSplit ? kSteps : 1][2];
+    // Queries: the B operand, lane (row col, channels 16 s + 8 half ..), requested
+    // ahead of the first tile and looked at when both are here. fp32 queries are
+    // scaled by a power of two to below 2^14 and split into two fp16 parts (22
+    // bits; the scale keeps the second part normal). Waves that have the same
+    // rows read a part of the channels each and share the fragments: four times
+    // 16 loads that touch 32 rows each held the first tile up (a prompt of 750
+    // rows spent 6000 cycles there).
+    constexpr int kMine = WR == 1 ? kSteps / kWaves : kSteps;
+    const int first_step = WR == 1 ? wave * kMine : 0;
+    s16x8 part[kSplit ? 2 : 1][kMine];
+    f32x4 raw[kSplit ? kMine : 1][2];
     float c = scale * kLog2e;
     {
       const Q* q = t.query(valid ? my_row : 0);
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
+      for (int s = 0; s < kMine; ++s) {
         // (Channels behind head_size are asked for at 0, and cleared below.)
-        const int d = 16 * s + 8 * half < size ? 16 * s + 8 * half : 0;
+        int d = 16 * (first_step + s) + 8 * half;
+        d = d < size ? d : 0;
         if constexpr (kSplit) {
           raw[s][0] = *reinterpret_cast<const f32x4*>(q + d);
           raw[s][1] = *reinterpret_cast<const f32x4*>(q + d + 4);
         } else {
-          qf[0][s] = *reinterpret_cast<const s16x8*>(q + d);
+          part[0][s] = *reinterpret_cast<const s16x8*>(q + d);
         }
       }
     }
@@ -292,24 +302,31 @@ struct Core {
     wait_loads();  // of the queries, as the compiler must know
     if (D != size) {
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-        if (16 * s + 8 * half >= size) {
+      for (int s = 0; s < kMine; ++s)
+        if (16 * (first_step + s) + 8 * half >= size) {
           if constexpr (kSplit) raw[s][0] = raw[s][1] = f32x4{};
-          else qf[0][s] = s16x8{};
+          else part[0][s] = s16x8{};
         }
     }
     if constexpr (kSplit) {
       float most = 0.0f;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s)
+      for (int s = 0; s < kMine; ++s)
 #pragma unroll
         for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(raw[s][j >> 2][j & 3]));
       most = fmaxf(most, other_half(most));
+      if constexpr (WR == 1) {
+        if (half == 0) marks[wave * 32 + col] = most;
+        lds_barrier();
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) most = fmaxf(most, marks[w * 32 + col]);
+        lds_barrier();
+      }
       const int e = (int)(f2u(most) >> 23) - 127;
       const int up = e == 128 ? 0 : clamp_int(13 - e, -114, 126);
       const float lift = u2f((unsigned)(up + 127) << 23);
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
+      for (int s = 0; s < kMine; ++s) {
         f16x8 hi, lo;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -317,10 +334,29 @@ struct Core {
           hi[j] = (_Float16)v;
           lo[j] = (_Float16)(v - (float)hi[j]);
         }
-        qf[0][s] = __builtin_bit_cast(s16x8, hi);
-        qf[kSplit ? 1 : 0][s] = __builtin_bit_cast(s16x8, lo);
+        part[0][s] = __builtin_bit_cast(s16x8, hi);
+        part[kSplit ? 1 : 0][s] = __builtin_bit_cast(s16x8, lo);
       }
       c = fmaxf(c * u2f((unsigned)(127 - up) << 23), 1.2e-38f);
+    }
+    s16x8 qf[kSplit ? 2 : 1][kSteps];
+    if constexpr (WR == 1) {
+      s16x8* shared = reinterpret_cast<s16x8*>(lds + kArea) + lane;
+#pragma unroll
+      for (int p = 0; p < (kSplit ? 2 : 1); ++p)
+#pragma unroll
+        for (int s = 0; s < kMine; ++s) shared[(p * kSteps + first_step + s) * 64] = part[p][s];
+      lds_barrier();
+#pragma unroll
+      for (int p = 0; p < (kSplit ? 2 : 1); ++p)
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) qf[p][s] = shared[(p * kSteps + s) * 64];
+      lds_barrier();  // the marks take their place
+    } else {
+#pragma unroll
+      for (int p = 0; p < (kSplit ? 2 : 1); ++p)
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) qf[p][s] = part[p][WR == 1 ? 0 : s];
     }
 
     f32x16 acc[D / 32];
@@ -541,7 +577,11 @@ struct Core {
       marks[(wave * 32 + col) * 2] = ref - kLift;
       marks[(wave * 32 + col) * 2 + 1] = total;
     }
-    const bool any_masked = __syncthreads_or(masked);
+    if (lane == 0) marks[64 * (kWaves + WR) + wave] = masked ? 1.0f : 0.0f;
+    __syncthreads();
+    bool any_masked = false;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) any_masked |= marks[64 * (kWaves + WR) + w] != 0.0f;
     float top = -kInf, sum = 0.0f, factor;
     {
       float m[WK];
@@ -680,7 +720,6 @@ template <typename Q, typename K, int D, int WR, int WK, int NK>
 __global__ __launch_bounds__(64 * WR * WK, 2) void packed_kernel(fah_packed_attention a, PackedCut cut) {
   using C = Core<Q, K, D, WR, WK, NK>;
   __shared__ __align__(16) unsigned char lds[C::kLds];
-  __shared__ float marks[C::kMarks];
   const int group = a.heads / a.kv_heads, head = blockIdx.x % a.kv_heads;
   const int rest = blockIdx.x / a.kv_heads, split = rest / (int)cut.slots, slot = (int)cut.slots - 1 - rest % (int)cut.slots;
   const PackedTile p = packed_tile(a, slot, group, C::BM);
@@ -718,7 +757,7 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void packed_kernel(fah_packed_atte
     sink.sums = static_cast<float*>(a.workspace) + item * C::BM * (D + 2);
     sink.marks = sink.sums + C::BM * D;
   }
-  C::run(t, sink, a.head_size, a.scale, lds, marks);
+  C::run(t, sink, a.head_size, a.scale, lds);
 }
 
 // Joins partial rows by groups of D / 4 lanes, four channels a lane: at(i) is
@@ -814,7 +853,6 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_kernel(fah_prefix_attentio
   using Own = Core<Q, K, D, 1, 4, 32>;
   static_assert(Shared::kThreads == kThreads && Own::kThreads == kThreads);
   __shared__ __align__(16) unsigned char lds[std::max(Shared::kLds, Own::kLds)];
-  __shared__ float marks[std::max(Shared::kMarks, Own::kMarks)];
   const int group = a.heads / a.kv_heads;
   float* partial = static_cast<float*>(a.workspace);
   Task<Q, K> t;
@@ -845,7 +883,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_kernel(fah_prefix_attentio
     const size_t rows = ((size_t)head * cut.shares + share_at) * all;
     sink.sums = partial + rows * (D + 2) + (size_t)row0 * D;
     sink.marks = partial + rows * (D + 2) + (size_t)all * D + 2 * row0;
-    C::run(t, sink, a.head_size, a.scale, lds, marks);
+    C::run(t, sink, a.head_size, a.scale, lds);
   } else {
     using C = Own;
     const int64_t at = blockIdx.x - cut.prefix_items;
@@ -890,7 +928,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_kernel(fah_prefix_attentio
       sink.sums = partial + rows * (D + 2) + (size_t)t.head0 * D;
       sink.marks = partial + rows * (D + 2) + (size_t)group * D + 2 * t.head0;
     }
-    C::run(t, sink, a.head_size, a.scale, lds, marks);
+    C::run(t, sink, a.head_size, a.scale, lds);
   }
 }
 
