@@ -88,6 +88,7 @@ internal static unsafe partial class Native
     [LibraryImport(Lib)] internal static partial int fah_decoder_decode(IntPtr decoder, float* embeddings, int frames, float* logits);
     [LibraryImport(Lib)] internal static partial int fah_decoder_embed(IntPtr decoder, int* tokens, int count, float* output);
     [LibraryImport(Lib)] internal static partial int fah_decoder_greedy(IntPtr decoder, out int token);
+    [LibraryImport(Lib)] internal static partial int fah_decoder_choose(IntPtr decoder, int* history, int historyCount, int promptCount, float repetition, float presence, float frequency, int* biasTokens, float* biasValues, int biasCount, uint* mask, float* logits, out int token);
     [LibraryImport(Lib)] internal static partial int fah_decoder_generate(IntPtr decoder, int steps, int* tokens);
     [LibraryImport(Lib)] internal static partial int fah_decoder_create_session(IntPtr parent, int capacity, out IntPtr session);
 

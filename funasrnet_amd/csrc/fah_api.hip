@@ -446,6 +446,7 @@ struct fah_decoder {
   int lm_groups = 0;
   int host_position = 0;
   bool have_logits = false;
+  bool logits_held = false;  // `logits` are those of the last step (a lock-step one keeps its own)
   bool fail_sessions = false;  // fah_decoder_fail_next_step: the next one-launch lock-step step fails too
   hipGraphExec_t graph_row = nullptr, graph_logits = nullptr, graph_step = nullptr;
   // Persistent single-launch step (one workgroup per CU), when the shape has
@@ -2557,7 +2558,7 @@ int fah_decoder_decode(fah_decoder* d, const float* embeddings, int frames, floa
     }
     recover_step_error(d);
     d->host_position += frames;
-    d->have_logits = logits != nullptr;
+    d->have_logits = d->logits_held = logits != nullptr;
     return FAH_OK;
   });
 }
@@ -2622,6 +2623,77 @@ int fah_decoder_generate(fah_decoder* d, int steps, int32_t* tokens) {
     }
     recover_step_error(d);
     d->host_position += steps;
+    if (steps > 0) d->logits_held = true;
+    return FAH_OK;
+  });
+}
+
+int fah_decoder_choose(fah_decoder* d, const int32_t* history, int history_count, int prompt_count, float repetition,
+                       float presence, float frequency, const int32_t* bias_tokens, const float* bias_values,
+                       int bias_count, const uint32_t* mask, float* logits, int32_t* token) {
+  if (!d || !token) return fail(FAH_ERROR_ARGUMENT, "decoder/token is NULL");
+  return guarded_decoder([&] {
+    require(history_count >= 0 && (history_count == 0 || history), "invalid history");
+    require(bias_count >= 0 && (bias_count == 0 || (bias_tokens && bias_values)), "invalid biases");
+    std::lock_guard<std::mutex> lock(d->ctx->gate);
+    require_live(d);
+    if (!d->have_logits) return fail(FAH_ERROR_STATE, "no logits: decode with logits first");
+    if (!d->logits_held) return fail(FAH_ERROR_STATE, "the last step was a lock-step one, which keeps no logits");
+    hipStream_t s = d->ctx->stream;
+    check(hipSetDevice(d->ctx->device), "hipSetDevice");
+    fah_logits_adjust call{};
+    call.logits = call.output = d->logits.ptr;
+    call.logits_stride = call.output_stride = call.vocab = d->cfg.vocab;
+    call.rows = 1;
+    call.type = FAH_TYPE_F32;
+    call.history_capacity = history_count;
+    call.bias_capacity = bias_count;
+    call.mask_rows = mask ? 1 : 0;
+    // One upload: the factors, the prompt's length and the lists, 16 bytes apart
+    // at least; behind them the choice and its workspace.
+    std::vector<uint8_t> blob;
+    auto put = [&](const void* from, size_t bytes) {
+      const size_t at = blob.size();
+      blob.resize(at + (bytes + 15) / 16 * 16);
+      if (bytes) std::memcpy(blob.data() + at, from, bytes);
+      return at;
+    };
+    const float factors[3] = {repetition, presence, frequency};
+    const size_t at_factors = put(factors, 12), at_prompt = put(&prompt_count, 4);
+    const size_t at_history = put(history, (size_t)history_count * 4), at_bias = put(bias_tokens, (size_t)bias_count * 4);
+    const size_t at_values = put(bias_values, (size_t)bias_count * 4);
+    const size_t at_mask = put(mask, mask ? ((size_t)d->cfg.vocab + 31) / 32 * 4 : 0);
+    int32_t chosen = -1;
+    call.tokens = &chosen;  // asked for (its place on the device follows)
+    const size_t at_token = blob.size(), workspace = (size_t)fah::logits_adjust_workspace(call);
+    {
+      DeviceWork work(*d->ctx);
+      d->staging.ensure(at_token + 16 + workspace);
+      char* base = d->staging.as<char>();
+      check(hipMemcpyAsync(base, blob.data(), blob.size(), hipMemcpyHostToDevice, s), "H2D lists");
+      call.repetition = reinterpret_cast<const float*>(base + at_factors);
+      call.presence = call.repetition + 1;
+      call.frequency = call.repetition + 2;
+      call.prompt_counts = reinterpret_cast<const int32_t*>(base + at_prompt);
+      call.history = reinterpret_cast<const int32_t*>(base + at_history);
+      call.bias_tokens = reinterpret_cast<const int32_t*>(base + at_bias);
+      call.bias_values = reinterpret_cast<const float*>(base + at_values);
+      call.masks = reinterpret_cast<const uint32_t*>(base + at_mask);
+      call.tokens = reinterpret_cast<int32_t*>(base + at_token);
+      call.workspace = base + at_token + 16;
+      call.workspace_bytes = (int64_t)workspace;
+      check(fah::launch_logits_adjust(call, s), "logits");
+      check(hipMemcpyAsync(&chosen, call.tokens, 4, hipMemcpyDeviceToHost, s), "D2H token");
+      if (logits)
+        check(hipMemcpyAsync(logits, d->logits.ptr, (size_t)d->cfg.vocab * 4, hipMemcpyDeviceToHost, s), "D2H logits");
+      check(hipStreamSynchronize(s), "hipStreamSynchronize");
+      if (chosen >= 0) {
+        check(hipMemcpyAsync(d->token.ptr, &chosen, 4, hipMemcpyHostToDevice, s), "H2D token");
+        check(hipStreamSynchronize(s), "hipStreamSynchronize");
+      }
+    }
+    if (chosen < 0) d->have_logits = false;  // no token to go on with
+    *token = chosen;
     return FAH_OK;
   });
 }
@@ -2714,7 +2786,10 @@ int fah_decoder_generate_sessions(fah_decoder* const* sessions, int count, int s
     if (work) work->release();  // enqueued: other contexts may enqueue while this stream drains
     check(hipStreamSynchronize(s), "hipStreamSynchronize");
     recover_session_step(b, sessions, count, s);
-    for (int i = 0; i < count; ++i) sessions[i]->host_position += steps;
+    for (int i = 0; i < count; ++i) {
+      sessions[i]->host_position += steps;
+      sessions[i]->logits_held = false;
+    }
     return FAH_OK;
   });
 }
@@ -2858,7 +2933,10 @@ void run_batch(fah_batcher* b, const std::vector<BatchRequest*>& reqs) {
                                   (unsigned)rb[fah::kFewFrames + 1], s);
     }
     check(hipStreamSynchronize(s), "hipStreamSynchronize");
-    for (fah_decoder* d : sessions) d->host_position += 1;
+    for (fah_decoder* d : sessions) {
+      d->host_position += 1;
+      d->logits_held = false;
+    }
     return FAH_OK;
   });
   const std::string message = status != FAH_OK ? fah_last_error() : std::string();

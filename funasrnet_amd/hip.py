@@ -151,6 +151,9 @@ SIGNATURES = {
     "fah_decoder_decode": (ctypes.c_int, [_vp, _f32p, ctypes.c_int, _f32p]),
     "fah_decoder_embed": (ctypes.c_int, [_vp, _i32p, ctypes.c_int, _f32p]),
     "fah_decoder_greedy": (ctypes.c_int, [_vp, _i32p]),
+    "fah_decoder_choose": (ctypes.c_int, [_vp, _i32p, ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_float,
+                                          ctypes.c_float, _i32p, _f32p, ctypes.c_int, ctypes.POINTER(ctypes.c_uint32),
+                                          _f32p, _i32p]),
     "fah_decoder_generate": (ctypes.c_int, [_vp, ctypes.c_int, _i32p]),
     "fah_decoder_create_session": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.POINTER(_vp)]),
     "fah_decoder_generate_sessions": (ctypes.c_int, [ctypes.POINTER(_vp), ctypes.c_int, ctypes.c_int, _i32p]),
@@ -592,6 +595,31 @@ class HipDecoder:
         v = ctypes.c_int32()
         _check(load().fah_decoder_greedy(self.handle, ctypes.byref(v)))
         return v.value
+
+    def choose(self, history=(), prompt: int = 0, repetition: float = 1.0, presence: float = 0.0, frequency: float = 0.0,
+               biases: dict | None = None, mask: np.ndarray | None = None, logits: np.ndarray | None = None) -> int:
+        """The greedy token of the last logits under penalties for the tokens of
+        `history` (its first `prompt` ones are the prompt), biases {token: value}
+        and a grammar's mask (a truth value per token); generate goes on with it.
+        -1: nothing is left. `logits` [vocab] receives the adjusted ones."""
+        h = np.ascontiguousarray(list(history), dtype=np.int32)
+        t = np.ascontiguousarray(list(biases or {}), dtype=np.int32)
+        v = np.ascontiguousarray(list((biases or {}).values()), dtype=np.float32)
+        words = None
+        if mask is not None:
+            if mask.shape != (self.config.vocab,):
+                raise ValueError("the mask needs a truth value for each token")
+            bits = np.zeros((self.config.vocab + 31) // 32 * 32, dtype=bool)
+            bits[:self.config.vocab] = mask
+            words = np.packbits(bits, bitorder="little").view(np.uint32)
+        if logits is not None and (logits.dtype != np.float32 or logits.size != self.config.vocab):
+            raise ValueError("logits must be float32 of the vocabulary's size")
+        token = ctypes.c_int32()
+        _check(load().fah_decoder_choose(self.handle, _p(h, ctypes.c_int32), h.size, prompt, repetition, presence, frequency,
+                                         _p(t, ctypes.c_int32), _p(v, ctypes.c_float), t.size,
+                                         None if words is None else _p(words, ctypes.c_uint32),
+                                         None if logits is None else _p(logits, ctypes.c_float), ctypes.byref(token)))
+        return token.value
 
     def generate(self, steps: int) -> np.ndarray:
         tokens = np.empty(max(steps, 1), dtype=np.int32)

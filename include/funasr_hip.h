@@ -455,6 +455,22 @@ int fah_decoder_embed(fah_decoder* decoder, const int32_t* tokens, int count, fl
  * last decode, computed on the device. */
 int fah_decoder_greedy(fah_decoder* decoder, int32_t* token);
 
+/* Greedy under penalties for repeated tokens, biases and a grammar's mask: the
+ * logits of the last decode or generate step are adjusted in place as
+ * fah_logits_adjust does it (one row, host lists; mask: (vocab + 31) / 32 words
+ * or NULL), and their choice is the token that fah_decoder_greedy returns and
+ * fah_decoder_generate goes on with. Adjusted logits are written to `logits`
+ * (host, [vocab]) when it is not NULL. *token is -1 when nothing is left to
+ * choose: the decoder then has no logits until it decodes again. A second call
+ * adjusts the adjusted logits. FAH_ERROR_STATE without logits and after a
+ * lock-step step, which keeps none. The loop of FunAsr.Transcribe
+ * (src/FunAsrNet/FunAsr.cs:167-178) with it: decode the prefix, then choose and
+ * generate one step in turn. No reference counterpart. */
+int fah_decoder_choose(fah_decoder* decoder, const int32_t* history, int history_count, int prompt_count,
+                       float repetition, float presence, float frequency, const int32_t* bias_tokens,
+                       const float* bias_values, int bias_count, const uint32_t* mask, float* logits,
+                       int32_t* token);
+
 /* The FunAsr.Transcribe loop (src/FunAsrNet/FunAsr.cs:167-178) without the
  * tokenizer's end check: `steps` times Greedy -> Embed -> Decode(1), entirely
  * on the device (token feedback stays in device memory; one persistent

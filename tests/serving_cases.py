@@ -51,6 +51,17 @@ def attend(q, k, v, scale, seen):
     return out, weight, dots
 
 
+def attend_all(q, k, v, scale, offset):
+    """attend() for many rows: row i sees the keys up to i + offset; finite values."""
+    q, k, v = (np.asarray(a, np.float64) for a in (q, k, v))
+    s = scale * (q @ k.T)
+    seen = np.arange(len(k))[None, :] <= np.arange(len(q))[:, None] + offset
+    top = np.where(seen, s, -np.inf).max(1, keepdims=True, initial=-np.inf)
+    p = np.where(seen, np.exp(s - np.where(np.isfinite(top), top, 0.0)), 0.0)
+    total = np.maximum(p.sum(1, keepdims=True), 1e-300)
+    return p @ v / total, p @ np.abs(v) / total, scale * (np.abs(q) @ np.abs(k).T).max(1, keepdims=True)
+
+
 def attention_bound(out, weight, dots, keys, size, kind):
     """How far a correct result may be off, from the roundings it makes:
     a score sums `size` products in 32 bits (size + 3 half steps of sum |q k|,

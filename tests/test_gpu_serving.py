@@ -4,7 +4,7 @@ token, at the sizes and masks where they can go wrong."""
 import numpy as np
 import pytest
 
-from serving_cases import CODES, adjusted, attend, attention_bound, load, store
+from serving_cases import CODES, adjusted, attend, attend_all, attention_bound, load, store
 
 pytestmark = pytest.mark.gpu
 
@@ -115,6 +115,217 @@ def test_packed(backend, types, queries, extra, heads, kv_heads, size):
     check_packed(got, q, k, v, qo, ko, types)
 
 
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(t))
+@pytest.mark.parametrize("queries,extra,heads,kv_heads,size", [
+    ([1100], [0], 64, 64, 128),             # 128 rows a workgroup
+    ([700, 3, 450], [0, 0, 0], 64, 64, 64),
+    ([400], [2500], 64, 64, 128),           # and the keys in shares
+    ([390], [2110], 64, 32, 96),
+    ([60, 45], [1500, 3000], 8, 4, 128),    # 64 rows, shares
+    ([1, 1, 1], [4000, 1200, 2600], 8, 8, 128),
+    ([7], [9000], 4, 1, 64),
+], ids=str)
+def test_packed_large(backend, types, queries, extra, heads, kv_heads, size):
+    keys = [a + b for a, b in zip(queries, extra)]
+    q, k, v = packed_inputs(sum(keys), queries, keys, heads, kv_heads, size, types)
+    qo, ko = offsets(queries), offsets(keys)
+    print(f"packed {queries} {extra} {heads}/{kv_heads} x {size} {types}", flush=True)
+    got = run_packed(backend, q, k, v, qo, ko, types)
+    fq, fk, fv, fg = load(q, types[0]), load(k, types[1]), load(v, types[1]), load(got, types[0])
+    for s in range(len(queries)):
+        (a, b), (c, d) = qo[s:s + 2], ko[s:s + 2]
+        for h in sorted({0, 1, heads // 2, heads - 1}):
+            g = h // (heads // kv_heads)
+            out, weight, dots = attend_all(fq[a:b, h], fk[c:d, g], fv[c:d, g], size**-0.5, extra[s])
+            off = np.abs(fg[a:b, h] - out)
+            limit = attention_bound(out, weight, dots, d - c, size, types[0])
+            assert np.all(off <= limit), (s, h, float((off / limit).max()))
+
+
+@pytest.mark.parametrize("count", [63, 64, 65, 300, 4200])
+def test_packed_many_sequences(backend, count):
+    """The search for a tile's sequence, with empty ones among them."""
+    rng = np.random.default_rng(count)
+    queries = rng.integers(0, 6, count).tolist()
+    keys = [a + int(b) for a, b in zip(queries, rng.integers(0, 3, count))]
+    types = ("f16", "f16")
+    q, k, v = packed_inputs(count, queries, keys, 2, 1, 64, types)
+    qo, ko = offsets(queries), offsets(keys)
+    got = run_packed(backend, q, k, v, qo, ko, types)
+    check_packed(got, q, k, v, qo, ko, types)
+
+
+def test_packed_rows_of_no_sequence_are_left(backend):
+    types = ("f32", "f16")
+    queries, keys = [20, 0, 33], [25, 4, 33]
+    q, k, v = packed_inputs(5, [70], [90], 4, 2, 128, types)
+    qo, ko = offsets(queries, 9), offsets(keys, 3)
+    keep = np.random.default_rng(1).standard_normal((70, 4 * 128)).astype(np.float32)
+    got = run_packed(backend, q, k, v, qo, ko, types, keep=keep)
+    check_packed(got, q, k, v, qo, ko, types)
+    kept = keep.reshape(70, 4, 128)
+    assert np.array_equal(got[:9], kept[:9]) and np.array_equal(got[9 + 53:], kept[9 + 53:])
+
+
+def test_packed_offsets_outside_the_rows(backend):
+    """Taken as the nearer end."""
+    types = ("f16", "f16")
+    q, k, v = packed_inputs(6, [50], [60], 2, 2, 64, types)
+    got = run_packed(backend, q, k, v, np.array([-7, 30, 1000], np.int32), np.array([-100, 40, 2**31 - 1], np.int32), types)
+    check_packed(got, q, k, v, np.array([0, 30, 50]), np.array([0, 40, 60]), types)
+
+
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(t))
+@pytest.mark.parametrize("rows,heads,kv_heads,extra", [(90, 2, 1, 0), (1100, 64, 64, 0), (400, 64, 64, 2500), (3, 4, 1, 700)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_packed_masked_places_may_hold_anything(backend, types, rows, heads, kv_heads, extra, bad):
+    """A late key and value only reach the rows that see them."""
+    keys = rows + extra
+    q, k, v = packed_inputs(rows, [rows], [keys], heads, kv_heads, 128, types)
+    at = keys - 2  # seen by the last two rows
+    plain = run_packed(backend, q, k, v, offsets([rows]), offsets([keys]), types)
+    spoilt_k, spoilt_v = k.copy(), v.copy()
+    spoilt_k[at] = store(np.full(spoilt_k[at].shape, bad), types[1])
+    spoilt_v[at] = store(np.full(spoilt_v[at].shape, bad), types[1])
+    got = load(run_packed(backend, q, spoilt_k, spoilt_v, offsets([rows]), offsets([keys]), types), types[0])
+    plain = load(plain, types[0])
+    # Rows before it: as without it, but for the order in which a row is summed.
+    limit = 2 * attention_bound(plain, np.abs(plain) + 4.0, 60.0, keys, 128, types[0])
+    assert np.all(np.isfinite(got[:rows - 2])) and np.all(np.abs(got[:rows - 2] - plain[:rows - 2]) <= limit[:rows - 2])
+    if bad != -np.inf:
+        assert not np.any(np.isfinite(got[rows - 2:]))
+
+
+def test_packed_row_of_minus_infinity_scores(backend):
+    types = ("f16", "f16")
+    q, k, v = packed_inputs(8, [40], [40], 2, 2, 64, types)
+    q[:] = store(np.abs(load(q, "f16")) + 0.1, "f16")
+    k[:3] = store(np.full((3, 2, 64), -np.inf), "f16")  # rows 0 to 2 only see these
+    got = load(run_packed(backend, q, k, v, offsets([40]), None, types), "f16")
+    assert np.all(got[:3] == 0)
+    fq, fk, fv = load(q, "f16"), load(k, "f16"), load(v, "f16")
+    for h in range(2):
+        out, weight, dots = attend_all(fq[3:, h], fk[3:, h], fv[3:, h], 64**-0.5, 0)
+        assert np.all(np.abs(got[3:, h] - out) <= attention_bound(out, weight, dots, 37, 64, "f16"))
+
+
+@pytest.mark.parametrize("magnitude", [1e-30, 1e-6, 1e4, 1e30])
+def test_packed_fp32_queries_of_any_size(backend, magnitude):
+    types = ("f32", "f16")
+    q, k, v = packed_inputs(9, [70], [70], 4, 2, 128, types)
+    q *= np.float32(magnitude)
+    scale = float(np.float32(128**-0.5 / magnitude))
+    got = run_packed(backend, q, k, v, offsets([70]), None, types, scale=scale)
+    check_packed(got, q, k, v, offsets([70]), None, types, scale=scale)
+
+
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(t))
+def test_packed_sharp_and_rising_scores(backend, types):
+    """Weights that differ by far, largest scores that keep rising."""
+    q, k, v = packed_inputs(10, [200], [200], 2, 1, 64, types)
+    k[:] = store(load(k, types[1]) * np.linspace(0.01, 12, 200)[:, None, None], types[1])
+    got = run_packed(backend, q, k, v, offsets([200]), None, types)
+    check_packed(got, q, k, v, offsets([200]), None, types)
+
+
+def test_packed_broadcast_and_cache_order(backend):
+    """One K/V head's rows for all (stride 0), and a cache with heads before rows."""
+    from funasrnet_amd import hip
+    types, heads, rows = ("f32", "f16"), 4, 45
+    q, k, v = packed_inputs(11, [rows], [rows], heads, 2, 128, types)
+    for shared in (True, False):
+        kk = np.repeat(k[:, :1], 2, 1) if shared else k
+        vv = np.repeat(v[:, :1], 2, 1) if shared else v
+        dk, dv = ((to_device(k[:, 0]), to_device(v[:, 0])) if shared else
+                  (to_device(np.swapaxes(k, 0, 1)), to_device(np.swapaxes(v, 0, 1))))
+        dq, out, do = to_device(q), to_device(np.zeros_like(q)), to_device(offsets([rows]))
+        head = 0 if shared else rows * 128
+        call = hip.PackedAttention(query=dq.ptr, key=dk.ptr, value=dv.ptr, output=out.ptr, query_row=heads * 128, query_head=128,
+                                   key_row=128, key_head=head, value_row=128, value_head=head, output_row=heads * 128,
+                                   output_head=128, query_offsets=do.ptr, sequences=1, query_rows=rows, key_rows=rows,
+                                   longest_query=rows, longest_key=rows, heads=heads, kv_heads=2, head_size=128,
+                                   query_type=hip.TYPE_F32, cache_type=hip.TYPE_F16, scale=128**-0.5)
+        assert backend.attention_packed_device(call) == hip.OK
+        backend.synchronize()
+        check_packed(out.numpy(), q, kk, vv, offsets([rows]), None, types)
+
+
+def test_packed_hints_only_steer(backend):
+    """Lengths beyond the hints are attended all the same."""
+    from funasrnet_amd import hip
+    types = ("bf16", "bf16")
+    q, k, v = packed_inputs(12, [300, 10], [1500, 1700], 4, 2, 128, types)
+    results = []
+    for longest in ((0, 0), (1, 1), (300, 1700), (100000, 100000)):
+        dq, dk, dv, out = to_device(q), to_device(k), to_device(v), to_device(np.zeros_like(q))
+        qo, ko = to_device(offsets([300, 10])), to_device(offsets([1500, 1700]))
+        call = hip.PackedAttention(query=dq.ptr, key=dk.ptr, value=dv.ptr, output=out.ptr, query_row=512, query_head=128,
+                                   key_row=256, key_head=128, value_row=256, value_head=128, output_row=512, output_head=128,
+                                   query_offsets=qo.ptr, key_offsets=ko.ptr, sequences=2, query_rows=310, key_rows=3200,
+                                   longest_query=longest[0], longest_key=longest[1], heads=4, kv_heads=2, head_size=128,
+                                   query_type=hip.TYPE_BF16, cache_type=hip.TYPE_BF16, scale=128**-0.5)
+        need = backend.attention_packed_workspace(call)
+        ws = workspace_of(need)
+        call.workspace, call.workspace_bytes = ws.ptr, need
+        assert backend.attention_packed_device(call) == hip.OK
+        backend.synchronize()
+        results.append(out.numpy())
+        check_packed(results[-1], q, k, v, offsets([300, 10]), offsets([1500, 1700]), types)
+
+
+def test_offsets_past_32_bits(backend):
+    """Keys and values more than 2^32 elements into their buffers."""
+    import ctypes
+    from funasrnet_amd import device, hip
+    rows, step = 40, (1 << 32) // 8 // 128 * 128  # 9 sequences, each half a Gi elements on
+    types = ("f16", "f16")
+    n = 9
+    arrays = prefix_inputs(13, n, 33, rows, 4, 2, 128, types)
+    q, pk, pv, k, v = arrays
+    big = [ctypes.c_void_p() for _ in range(2)]
+    run = device.runtime()
+    lengths = np.full(n, rows, np.int32)
+    try:
+        for p, a in zip(big, (k, v)):
+            assert run.hipMalloc(ctypes.byref(p), (step * n) * 2) == 0
+            for s in range(n):
+                block = np.ascontiguousarray(a[s])
+                assert run.hipMemcpy(p.value + s * step * 2, block.ctypes.data, block.nbytes, device.H2D) == 0
+        dq, dpk, dpv, dl, out = to_device(q), to_device(pk), to_device(pv), to_device(lengths), to_device(np.zeros_like(q))
+        call = hip.PrefixAttention(
+            query=dq.ptr, prefix_key=dpk.ptr, prefix_value=dpv.ptr, key=big[0].value, value=big[1].value, output=out.ptr,
+            lengths=dl.ptr, query_sequence=512, query_head=128, prefix_key_row=256, prefix_key_head=128, prefix_value_row=256,
+            prefix_value_head=128, key_sequence=step, key_row=256, key_head=128, value_sequence=step, value_row=256,
+            value_head=128, output_sequence=512, output_head=128, sequences=n, prefix=33, capacity=rows, longest=rows, heads=4,
+            kv_heads=2, head_size=128, query_type=hip.TYPE_F16, cache_type=hip.TYPE_F16, scale=128**-0.5)
+        need = backend.attention_prefix_workspace(call)
+        ws = workspace_of(need)
+        call.workspace, call.workspace_bytes = ws.ptr, need
+        assert backend.attention_prefix_device(call) == hip.OK
+        backend.synchronize()
+        check_prefix(out.numpy(), *arrays, lengths, types)
+        # The last sequence's rows as a packed prompt whose rows are 2^24 elements apart.
+        far = 1 << 24
+        for p, a in zip(big, (k, v)):
+            for r in range(rows):
+                block = np.ascontiguousarray(a[n - 1, r])
+                assert run.hipMemcpy(p.value + r * far * 2, block.ctypes.data, block.nbytes, device.H2D) == 0
+        qq = np.ascontiguousarray(np.resize(q, (rows, 4, 128)))
+        dq, out, do = to_device(qq), to_device(np.zeros_like(qq)), to_device(offsets([rows]))
+        call = hip.PackedAttention(query=dq.ptr, key=big[0].value, value=big[1].value, output=out.ptr, query_row=512,
+                                   query_head=128, key_row=far, key_head=128, value_row=far, value_head=128, output_row=512,
+                                   output_head=128, query_offsets=do.ptr, sequences=1, query_rows=rows, key_rows=rows,
+                                   longest_query=rows, longest_key=rows, heads=4, kv_heads=2, head_size=128,
+                                   query_type=hip.TYPE_F16, cache_type=hip.TYPE_F16, scale=128**-0.5)
+        assert backend.attention_packed_device(call) == hip.OK
+        backend.synchronize()
+        check_packed(out.numpy(), qq, k[n - 1], v[n - 1], offsets([rows]), None, types)
+    finally:
+        for p in big:
+            if p.value:
+                run.hipFree(p.value)
+
+
 # ---- A shared prefix ----------------------------------------------------------------
 
 
@@ -195,6 +406,63 @@ def test_prefix(backend, types, lengths, prefix, capacity, heads, kv_heads, size
     for heads_first in (True, False):
         got = run_prefix(backend, *arrays, lengths, types, heads_first=heads_first)
         check_prefix(got, *arrays, lengths, types)
+
+
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(t))
+@pytest.mark.parametrize("count,prefix,longest,heads,kv_heads,size", [
+    (300, 700, 90, 16, 8, 64),       # 64 rows of the prefix a workgroup
+    (1100, 130, 5, 64, 8, 8),        # 128
+    (40, 1500, 900, 8, 4, 128),      # own rows in one share
+    (2, 4000, 3000, 4, 2, 128),      # and in several
+    (70, 65, 40, 40, 1, 128),        # more heads a group than a tile has rows
+], ids=str)
+def test_prefix_large(backend, types, count, prefix, longest, heads, kv_heads, size):
+    rng = np.random.default_rng(count)
+    lengths = rng.integers(0, longest + 1, count)
+    arrays = prefix_inputs(count, count, prefix, longest, heads, kv_heads, size, types)
+    print(f"prefix {count} {prefix} {longest} {heads}/{kv_heads} x {size} {types}", flush=True)
+    got = run_prefix(backend, *arrays, lengths, types)
+    some = np.unique(np.concatenate([rng.integers(0, count, 25), [0, count - 1]]))
+    check_prefix(got[some], arrays[0][some], *arrays[1:3], arrays[3][some], arrays[4][some], lengths[some], types)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_prefix_rows_behind_the_length_may_hold_anything(backend, bad):
+    types = ("f32", "f16")
+    lengths = [0, 1, 31, 32, 33, 100]
+    for prefix in (0, 50, 1500):
+        q, pk, pv, k, v = prefix_inputs(prefix + 3, len(lengths), prefix, 128, 4, 2, 128, types)
+        for s, n in enumerate(lengths):
+            k[s, n:] = bad
+            v[s, n:] = bad
+        got = run_prefix(backend, q, pk, pv, k, v, lengths, types)
+        check_prefix(got, q, pk, pv, k, v, lengths, types)
+
+
+@pytest.mark.parametrize("prefix", [300, 2000])
+def test_prefix_value_that_is_infinite(backend, prefix):
+    """An infinite value reaches every row, a NaN of one sequence that one alone."""
+    types = ("bf16", "bf16")
+    q, pk, pv, k, v = prefix_inputs(4, 5, prefix, 64, 4, 2, 64, types)
+    lengths = [64, 3, 50, 0, 20]
+    v[2, 7, 1] = store(np.full(64, np.nan), "bf16")
+    pv[11, 0] = store(np.full(64, np.inf), "bf16")
+    got = load(run_prefix(backend, q, pk, pv, k, v, lengths, types), "bf16")
+    assert np.all(got[:, :2] == np.inf)
+    assert np.all(np.isnan(got[2, 2:])) and np.all(np.isfinite(got[[0, 1, 3, 4], 2:]))
+
+
+def test_attention_is_deterministic(backend):
+    types = ("f32", "f16")
+    arrays = prefix_inputs(5, 20, 1800, 400, 8, 4, 128, types)
+    lengths = np.random.default_rng(5).integers(0, 400, 20)
+    first = run_prefix(backend, *arrays, lengths, types)
+    q, k, v = packed_inputs(6, [300, 40], [1800, 2500], 8, 4, 128, types)
+    packed = run_packed(backend, q, k, v, offsets([300, 40]), offsets([1800, 2500]), types)
+    for _ in range(3):
+        assert np.array_equal(first.view(np.uint32), run_prefix(backend, *arrays, lengths, types).view(np.uint32))
+        again = run_packed(backend, q, k, v, offsets([300, 40]), offsets([1800, 2500]), types)
+        assert np.array_equal(packed.view(np.uint32), again.view(np.uint32))
 
 
 # ---- The choice of a token ------------------------------------------------------------
@@ -292,3 +560,341 @@ def test_choice(backend, kind, rows, vocab, history, biases, masks, pad):
     assert np.array_equal(got.view(np.uint8), again.view(np.uint8)) and np.array_equal(picked, same)
     alone, _ = run_choice(backend, v, kind, pad, tokens=False)
     assert np.array_equal(got.view(np.uint8), alone.view(np.uint8))
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_choice_of_unusual_values(backend, kind):
+    v = choice_inputs(3, 6, 700, 30, 5, 0, kind)
+    x = load(v["logits"], kind)
+    x[0, ::3] = np.nan
+    x[1] = -np.inf
+    x[2, 5], x[2, 600] = np.inf, np.inf
+    x[3] = np.nan
+    x[4] = -0.0
+    x[4, 300] = 0.0
+    v["logits"] = store(x, kind)
+    v["counts"][:] = [30, 0, 30, 30, 0, 30]
+    v["bias_counts"][:] = [5, 0, 0, 0, 0, 5]
+    got, picked = run_choice(backend, v, kind)
+    check_choice(got, picked, v, kind)
+    assert picked[1] == -1 and picked[3] == -1 and picked[4] == 0
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_choice_lists_and_masks_shared_by_rows(backend, kind):
+    """Stride 0 lists, one mask for all, no index, no counts, unaligned and differently aligned rows."""
+    from funasrnet_amd import hip
+    from funasrnet_amd.device import DeviceArray
+    rng = np.random.default_rng(17)
+    rows, vocab = 5, 3001
+    v = choice_inputs(18, rows, vocab, 12, 4, 1, kind)
+    v["masks"][0] = rng.integers(0, 1 << 32, v["masks"].shape[1], dtype=np.uint64)
+    for lead_in, lead_out in ((0, 0), (1, 1), (3, 2), (5, 0)):
+        width = 4 if kind == "f32" else 2
+        wide = np.full(rows * (vocab + 6) + 8, 3, v["logits"].dtype)
+        for r in range(rows):
+            wide[lead_in + r * (vocab + 6):][:vocab] = v["logits"][r]
+        logits, out = to_device(wide), to_device(np.full_like(wide, 4))
+        chosen = DeviceArray(rows, np.int32)
+        held = {n: to_device(a[0] if n in ("history", "bias_tokens", "bias_values") else a) for n, a in v.items() if n != "logits"}
+        call = hip.LogitsAdjust(logits=logits.ptr + lead_in * width, output=out.ptr + lead_out * width, tokens=chosen.ptr,
+                                logits_stride=vocab + 6, output_stride=vocab + 6, rows=rows, vocab=vocab, type=CODES[kind],
+                                history=held["history"].ptr, history_stride=0, history_capacity=12,
+                                repetition=held["repetition"].ptr, bias_tokens=held["bias_tokens"].ptr,
+                                bias_values=held["bias_values"].ptr, bias_stride=0, bias_capacity=4, masks=held["masks"].ptr,
+                                mask_stride=v["masks"].shape[1], mask_rows=1)
+        need = backend.logits_adjust_workspace(call)
+        ws = workspace_of(need)
+        call.workspace, call.workspace_bytes = ws.ptr, need
+        assert backend.logits_adjust_device(call) == hip.OK
+        backend.synchronize()
+        got, picked = out.numpy(), chosen.numpy()
+        mask = np.unpackbits(v["masks"][0].view(np.uint8), bitorder="little")[:vocab] == 1
+        for r in range(rows):
+            bias = list(zip(v["bias_tokens"][0].tolist(), v["bias_values"][0]))
+            expected, token = adjusted(load(v["logits"][r], kind), v["history"][0].tolist(), 0, v["repetition"][r], 0, 0, bias,
+                                       mask, kind)
+            row = got[lead_out + r * (vocab + 6):]
+            assert np.array_equal(row[:vocab].view(np.uint8), expected.view(np.uint8)) and picked[r] == token
+            assert np.all(row[vocab:vocab + 6] == 4)
+
+
+def test_choice_counts_out_of_range(backend):
+    """Counts below 0 and above the capacity, prompts longer than the history."""
+    v = choice_inputs(19, 4, 500, 20, 6, 0, "f32")
+    v["counts"][:] = [-3, 21, 20, 2**31 - 1]
+    v["prompts"][:] = [0, -5, 2**31 - 1, 3]
+    v["bias_counts"][:] = [7, -1, 2**31 - 1, 0]
+    got, picked = run_choice(backend, v, "f32")
+    v["counts"][:] = [0, 20, 20, 20]
+    v["bias_counts"][:] = [6, 0, 6, 0]
+    check_choice(got, picked, v, "f32")
+
+
+# ---- Refusals that need a context -----------------------------------------------------
+
+
+def test_refusals_with_a_context(backend):
+    from funasrnet_amd import hip
+    lib = hip.load()
+    import ctypes
+    types = ("f32", "f16")
+    q, k, v = packed_inputs(1, [4], [3000], 2, 1, 128, types)
+    dq, dk, dv, out = to_device(q), to_device(k), to_device(v), to_device(np.full_like(q, 5))
+    qo, ko = to_device(offsets([4])), to_device(offsets([3000]))
+
+    def call(**changes):
+        a = hip.PackedAttention(query=dq.ptr, key=dk.ptr, value=dv.ptr, output=out.ptr, query_row=256, query_head=128,
+                                key_row=128, key_head=128, value_row=128, value_head=128, output_row=256, output_head=128,
+                                query_offsets=qo.ptr, key_offsets=ko.ptr, sequences=1, query_rows=4, key_rows=3000,
+                                longest_query=4, longest_key=3000, heads=2, kv_heads=1, head_size=128,
+                                query_type=hip.TYPE_F32, cache_type=hip.TYPE_F16, scale=0.1)
+        need = backend.attention_packed_workspace(a)
+        assert need > 0
+        a.workspace_bytes = need
+        for name, value in changes.items():
+            setattr(a, name, value)
+        return lib.fah_attention_packed_device(backend.handle, ctypes.byref(a))
+
+    ws = workspace_of(1 << 22)
+    assert call() == hip.ERROR_ARGUMENT and b"workspace" in lib.fah_last_error()          # none given
+    assert call(workspace=ws.ptr, workspace_bytes=16) == hip.ERROR_ARGUMENT               # too small
+    assert call(workspace=ws.ptr + 4) == hip.ERROR_ARGUMENT                               # off its boundary
+    for name in ("query", "key", "value", "output", "query_offsets"):
+        assert call(workspace=ws.ptr, **{name: None}) == hip.ERROR_ARGUMENT, name
+    for name, at in (("query", dq.ptr), ("key", dk.ptr), ("value", dv.ptr), ("output", out.ptr)):
+        assert call(workspace=ws.ptr, **{name: at + 2}) == hip.DECLINED, name
+    assert np.all(out.numpy() == 5)
+    assert call(workspace=ws.ptr, sequences=0) == hip.OK and call(workspace=ws.ptr, query_rows=0) == hip.OK
+    backend.synchronize()
+    assert np.all(out.numpy() == 5)
+    a = hip.LogitsAdjust(logits=dq.ptr, output=out.ptr, logits_stride=100, output_stride=100, rows=2, vocab=100)
+    for changes in (dict(logits=None), dict(output=None), dict(output_stride=99), dict(logits=dq.ptr + 2),
+                    dict(history_capacity=1), dict(bias_capacity=1), dict(mask_rows=1), dict(logits=out.ptr, logits_stride=128),
+                    dict(vocab=0), dict(tokens=qo.ptr)):
+        b = hip.LogitsAdjust.from_buffer_copy(a)
+        for name, value in changes.items():
+            setattr(b, name, value)
+        assert lib.fah_logits_adjust_device(backend.handle, ctypes.byref(b)) == hip.ERROR_ARGUMENT, changes
+    assert np.all(out.numpy() == 5)
+
+
+# ---- Together, in graphs, on threads -----------------------------------------------------
+
+
+class Serving:
+    """A batch behind a shared prefix: its prompts, a decode step and the choice of a token."""
+
+    def __init__(self, backend, seed, count=6, prefix=600, own=70, heads=8, kv_heads=4, vocab=4000):
+        from funasrnet_amd import hip
+        from funasrnet_amd.device import DeviceArray
+        self.backend, self.types, size = backend, ("f32", "f16"), 128
+        rng = np.random.default_rng(seed)
+        self.q, self.pk, self.pv, self.k, self.v = prefix_inputs(seed, count, prefix, own, heads, kv_heads, size, self.types)
+        self.lengths = rng.integers(1, own + 1, count).astype(np.int32)
+        self.choice = choice_inputs(seed, count, vocab, 40, 8, 3, "f32")
+        self.hold = {n: to_device(a) for n, a in dict(q=self.q, pk=self.pk, pv=self.pv, k=self.k, v=self.v, lengths=self.lengths,
+                                                      **self.choice).items()}
+        d = self.hold
+        self.out, self.adjusted = DeviceArray(self.q.shape, np.float32), DeviceArray((count, vocab), np.float32)
+        self.tokens = DeviceArray(count, np.int32)
+        row = kv_heads * size
+        self.attend = hip.PrefixAttention(
+            query=d["q"].ptr, prefix_key=d["pk"].ptr, prefix_value=d["pv"].ptr, key=d["k"].ptr, value=d["v"].ptr,
+            output=self.out.ptr, lengths=d["lengths"].ptr, query_sequence=heads * size, query_head=size, prefix_key_row=row,
+            prefix_key_head=size, prefix_value_row=row, prefix_value_head=size, key_sequence=own * row, key_row=row,
+            key_head=size, value_sequence=own * row, value_row=row, value_head=size, output_sequence=heads * size,
+            output_head=size, sequences=count, prefix=prefix, capacity=own, longest=own, heads=heads, kv_heads=kv_heads,
+            head_size=size, query_type=hip.TYPE_F32, cache_type=hip.TYPE_F16, scale=size**-0.5)
+        self.pick = hip.LogitsAdjust(
+            logits=d["logits"].ptr, output=self.adjusted.ptr, tokens=self.tokens.ptr, logits_stride=vocab, output_stride=vocab,
+            rows=count, vocab=vocab, type=hip.TYPE_F32, history=d["history"].ptr, history_stride=40, history_capacity=40,
+            history_counts=d["counts"].ptr, prompt_counts=d["prompts"].ptr, repetition=d["repetition"].ptr,
+            presence=d["presence"].ptr, frequency=d["frequency"].ptr, bias_tokens=d["bias_tokens"].ptr,
+            bias_values=d["bias_values"].ptr, bias_stride=8, bias_capacity=8, bias_counts=d["bias_counts"].ptr,
+            masks=d["masks"].ptr, mask_stride=self.choice["masks"].shape[1], mask_rows=3, mask_index=d["index"].ptr)
+        # The prefix's own rows as a packed prompt, with the first sequence's queries repeated.
+        self.prompt_q = np.ascontiguousarray(np.resize(self.q, (prefix, heads, size)))
+        self.prompt_out = DeviceArray(self.prompt_q.shape, np.float32)
+        self.hold["prompt_q"], self.hold["offsets"] = to_device(self.prompt_q), to_device(offsets([prefix]))
+        self.prompt = hip.PackedAttention(
+            query=d["prompt_q"].ptr, key=d["pk"].ptr, value=d["pv"].ptr, output=self.prompt_out.ptr, query_row=heads * size,
+            query_head=size, key_row=row, key_head=size, value_row=row, value_head=size, output_row=heads * size,
+            output_head=size, query_offsets=d["offsets"].ptr, sequences=1, query_rows=prefix, key_rows=prefix,
+            longest_query=prefix, longest_key=prefix, heads=heads, kv_heads=kv_heads, head_size=size,
+            query_type=hip.TYPE_F32, cache_type=hip.TYPE_F16, scale=size**-0.5)
+        self.spaces = []
+        for a, need in ((self.attend, backend.attention_prefix_workspace(self.attend)),
+                        (self.pick, backend.logits_adjust_workspace(self.pick)),
+                        (self.prompt, backend.attention_packed_workspace(self.prompt))):
+            self.spaces.append(workspace_of(need))
+            a.workspace, a.workspace_bytes = self.spaces[-1].ptr, need
+
+    def enqueue(self):
+        from funasrnet_amd import hip
+        assert self.backend.attention_packed_device(self.prompt) == hip.OK
+        assert self.backend.attention_prefix_device(self.attend) == hip.OK
+        assert self.backend.logits_adjust_device(self.pick) == hip.OK
+
+    def results(self):
+        return self.prompt_out.numpy(), self.out.numpy(), self.adjusted.numpy(), self.tokens.numpy()
+
+    def clear(self):
+        for a in (self.prompt_out, self.out, self.adjusted, self.tokens):
+            a.fill_zero()
+        for a in self.spaces:
+            a.upload(np.full(a.shape, 0xFF, np.uint8))
+
+    def check(self):
+        prompt, out, logits, tokens = self.results()
+        check_packed(prompt, self.prompt_q, self.pk, self.pv, offsets([len(self.pk)]), None, self.types)
+        check_prefix(out, self.q, self.pk, self.pv, self.k, self.v, self.lengths, self.types)
+        check_choice(logits, tokens, self.choice, "f32")
+
+
+def same(a, b):
+    return all(np.array_equal(x.view(np.uint8), y.view(np.uint8)) for x, y in zip(a, b))
+
+
+def test_a_serving_step(backend):
+    """Prompts, decode behind the prefix, choice, one behind the other on the context's stream."""
+    s = Serving(backend, 21)
+    s.clear()
+    s.enqueue()
+    backend.synchronize()
+    s.check()
+    # A sequence that decodes the last row of its own prompt gets that row's result.
+    n, heads = int(s.lengths[0]), s.q.shape[1]
+    k = np.concatenate([s.pk, s.k[0, :n]])
+    v = np.concatenate([s.pv, s.v[0, :n]])
+    queries = np.ascontiguousarray(np.resize(s.q, (n, heads, 128)))
+    queries[-1] = s.q[0]
+    got = run_packed(backend, queries, k, v, offsets([n]), offsets([len(k)]), s.types)
+    assert np.abs(got[-1] - s.results()[1][0]).max() < 1e-5
+
+
+def test_graphs_replay_the_calls(backend):
+    """Two graphs with workspaces of their own, replayed several times with other
+    work and changed inputs between, against the calls made one by one."""
+    import ctypes
+    from funasrnet_amd import device
+    run = device.runtime()
+    vp = ctypes.c_void_p
+    both = [Serving(backend, 31), Serving(backend, 32, count=3, prefix=2500, own=300)]
+    graphs = []
+    for s in both:
+        s.enqueue()  # once before, as a program warms up
+        backend.synchronize()
+        graph, made = vp(), vp()
+        assert run.hipStreamBeginCapture(vp(backend.stream), 2) == 0  # relaxed
+        s.enqueue()
+        assert run.hipStreamEndCapture(vp(backend.stream), ctypes.byref(graph)) == 0
+        assert run.hipGraphInstantiate(ctypes.byref(made), graph, None, None, ctypes.c_size_t(0)) == 0
+        graphs.append((graph, made))
+    rng = np.random.default_rng(33)
+    for turn in range(4):
+        for s in both:
+            s.q = (rng.standard_normal(s.q.shape) * 1.5).astype(np.float32)
+            s.lengths = rng.integers(1, s.k.shape[1] + 1, len(s.lengths)).astype(np.int32)
+            s.hold["q"].upload(s.q)
+            s.hold["lengths"].upload(s.lengths)
+            s.clear()
+        for _, made in graphs:
+            assert run.hipGraphLaunch(made, vp(backend.stream)) == 0
+        backend.synchronize()
+        replayed = [s.results() for s in both]
+        for s, r in zip(both, replayed):
+            s.check()
+            s.clear()
+            s.enqueue()
+            backend.synchronize()
+            assert same(r, s.results()), turn
+    for graph, made in graphs:
+        run.hipGraphExecDestroy(made)
+        run.hipGraphDestroy(graph)
+
+
+def test_two_contexts_on_two_threads():
+    import threading
+    from funasrnet_amd.hip import HipBackend
+    backends = [HipBackend(0), HipBackend(0)]
+    try:
+        work = [Serving(b, 41 + i, count=5 + i) for i, b in enumerate(backends)]
+        for s in work:
+            s.enqueue()
+            s.backend.synchronize()
+        alone = [s.results() for s in work]
+        for s in work:
+            s.clear()
+        errors = []
+
+        def turn(s, expected):
+            try:
+                for _ in range(30):
+                    s.enqueue()
+                    s.backend.synchronize()
+                if not same(expected, s.results()):
+                    errors.append("results differ")
+            except Exception as e:  # reported below
+                errors.append(repr(e))
+
+        threads = [threading.Thread(target=turn, args=(s, r)) for s, r in zip(work, alone)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join(timeout=60)
+        assert not any(t.is_alive() for t in threads) and not errors, errors
+    finally:
+        for b in backends:
+            b.close()
+
+
+# ---- The decoder's own loop -----------------------------------------------------------
+
+
+@pytest.mark.parametrize("persistent", ["1", "0"])
+def test_decoder_choose(persistent, monkeypatch, oracle_lib):
+    """choose() adjusts the step's logits, and generate() goes on with its token."""
+    from funasrnet_amd import hip, model
+    monkeypatch.setenv("FAH_PERSISTENT", persistent)
+    weights = model.synthetic(model.small_config(layers=2, vocab=2048), seed=3)
+    x = np.random.default_rng(0).standard_normal((6, weights.config.width)).astype(np.float32)
+    backend = hip.HipBackend(0)
+    gpu, ref = hip.HipDecoder(backend, weights, capacity=64), oracle_lib.Decoder(weights, capacity=64)
+    try:
+        with pytest.raises(RuntimeError, match="no logits"):
+            gpu.choose()
+        logits = gpu.decode(x, 6)
+        expected = ref.decode(x, 6)
+        rng = np.random.default_rng(7)
+        written, prompt = [5, 9, 5], 2
+        for step in range(8):
+            mask = rng.random(2048) < 0.7
+            biases = {int(t): float(b) for t, b in zip(rng.integers(0, 2048, 4), rng.uniform(-2, 2, 4))}
+            seen = np.empty(2048, np.float32)
+            token = gpu.choose(written, prompt, 1.3, 0.4, 0.2, biases, mask, seen)
+            want, choice = adjusted(logits, written, prompt, 1.3, 0.4, 0.2, list(biases.items()), mask, "f32")
+            assert np.array_equal(seen.view(np.uint32), want.view(np.uint32)) and token == choice
+            assert gpu.greedy() == token
+            # Its row's logits: the oracle's after the same token.
+            assert gpu.generate(1).tolist() == [token]
+            expected = ref.decode(ref.embed([token]), 1)
+            written.append(token)
+            logits = np.empty(2048, np.float32)
+            gpu.choose(logits=logits)  # as they are
+            assert np.abs(logits - expected).max() < 1e-2
+        assert gpu.position == 6 + 8
+        # Nothing left to choose.
+        assert gpu.choose(mask=np.zeros(2048, bool)) == -1
+        with pytest.raises(RuntimeError, match="no logits"):
+            gpu.generate(1)
+        gpu.set_position(6)
+        gpu.decode(x[:1], 1)
+        # A lock-step step keeps no logits.
+        hip.HipDecoder.generate_sessions([gpu], 1)
+        with pytest.raises(RuntimeError, match="lock-step"):
+            gpu.choose()
+    finally:
+        gpu.close()
+        ref.close()
+        backend.close()
