@@ -60,11 +60,6 @@ struct Task {
   int begin, end;            // keys
   int first_limit;           // token 0 sees the keys below this; per token one more if causal
   bool causal;
-  // A second range, the keys [0, more_end) of other rows, which every token
-  // sees (one group of rows only; 0: none).
-  const K *more_k, *more_v;
-  unsigned more_k_row, more_v_row;
-  int more_end;
   // Row r's token and head. (r + head0 is below 2^20: the product is within a
   // quarter of the exact quotient, which is at least half a step from a whole
   // number's edge.)
@@ -183,15 +178,13 @@ struct Loader {
 // The lane's two sums, then the row's reference and total.
 template <typename Q, typename K>
 __device__ __noinline__ f32x4 slow_row(const Q* q, const K* k_rows, const K* v_rows, unsigned k_row, unsigned v_row, int begin,
-                                       int lim, const K* more_k, const K* more_v, unsigned more_k_row, unsigned more_v_row,
-                                       int more_end, int size, float scale) {
-  const int lane = threadIdx.x & 63, count = lim > begin ? lim - begin : 0;
+                                       int lim, int size, float scale) {
+  const int lane = threadIdx.x & 63;
   float x[2] = {}, sum[2] = {}, top = -kInf, total = 0.0f;
   for (int i = 0; i < 2; ++i)
     if (2 * lane + i < size) x[i] = (float)q[2 * lane + i];
-  for (int n = 0; n < count + more_end; ++n) {
-    const K* k = n < count ? k_rows + (int64_t)(begin + n) * k_row : more_k + (int64_t)(n - count) * more_k_row;
-    const K* w = n < count ? v_rows + (int64_t)(begin + n) * v_row : more_v + (int64_t)(n - count) * more_v_row;
+  for (int key = begin; key < lim; ++key) {
+    const K *k = k_rows + (int64_t)key * k_row, *w = v_rows + (int64_t)key * v_row;
     float s = 0.0f, v[2] = {};
     for (int i = 0; i < 2; ++i)
       if (2 * lane + i < size) {
@@ -248,9 +241,9 @@ struct Core {
     const int wr = wave / WK, wk = wave % WK;
     const int my_row = wr * 32 + col;
     const bool valid = my_row < t.rows;
-    int lim = valid ? t.limit(my_row) : 0;
+    const int lim = valid ? t.limit(my_row) : 0;
     const int wave_rows = clamp_int(t.rows - wr * 32, 0, 32);
-    int lim_low = wave_rows ? (int)uniform(t.limit(wr * 32)) : 0;
+    const int lim_low = wave_rows ? (int)uniform(t.limit(wr * 32)) : 0;
     const int lim_high = wave_rows ? (int)uniform(t.limit(wr * 32 + wave_rows - 1)) : 0;
     const int end = (int)uniform(t.limit(t.rows - 1));  // of the workgroup
     const int last = t.end - 1;
@@ -454,40 +447,18 @@ struct Core {
     if constexpr (WR == 1) {
       // The next keys are on their way from the moment these are read, the next
       // values likewise: one buffer, and no wave waits for another.
-      const K *k = t.k, *v = t.v;
-      unsigned k_row = t.k_row, v_row = t.v_row;
-      int from = wave_begin, to = wave_end, at_most = last;
-      KeyLoader keys = key_loader;
-      ValueLoader values = value_loader;
-      for (bool more_rows = t.more_end > 0;; more_rows = false) {
-        for (int key = from; key < to; key += TR) {
-          const bool more = key + TR < to;
-          wait_loads_but<ValueLoader::kLoads>();
-          score(0);
-          wait_reads();
-          if (more) keys.load(k, k_row, key + TR, at_most, 0, size);
-          weigh(key);
-          if (more) wait_loads_but<KeyLoader::kLoads>();
-          else wait_loads_but<0>();
-          collect(0);
-          wait_reads();
-          if (more) values.load(v, v_row, key + TR, at_most, 0, size);
-        }
-        if (!more_rows) break;
-        k = t.more_k;
-        v = t.more_v;
-        k_row = t.more_k_row;
-        v_row = t.more_v_row;
-        from = wk * NK;
-        to = lim_low = t.more_end;
-        lim = valid ? t.more_end : 0;
-        at_most = t.more_end - 1;
-        keys = KeyLoader(lds + own * T::kRowBytes, k_row, loader);
-        values = ValueLoader(lds + kTileBytes + own * T::kRowBytes, v_row, loader);
-        if (from < to) {
-          keys.load(k, k_row, from, at_most, 0, size);
-          values.load(v, v_row, from, at_most, 0, size);
-        }
+      for (int key = wave_begin; key < wave_end; key += TR) {
+        const bool more = key + TR < wave_end;
+        wait_loads_but<ValueLoader::kLoads>();
+        score(0);
+        wait_reads();
+        if (more) key_loader.load(t.k, t.k_row, key + TR, last, 0, size);
+        weigh(key);
+        if (more) wait_loads_but<KeyLoader::kLoads>();
+        else wait_loads_but<0>();
+        collect(0);
+        wait_reads();
+        if (more) value_loader.load(t.v, t.v_row, key + TR, last, 0, size);
       }
     } else {
       // Two buffers. The barrier: this one's tile is here, and the other one's
@@ -555,8 +526,7 @@ struct Core {
       }
       for (unsigned rows_bad = (unsigned)__builtin_amdgcn_ballot_w64(bad); rows_bad != 0; rows_bad &= rows_bad - 1) {
         const int r = wr * 32 + __builtin_ctz(rows_bad);
-        const f32x4 v = slow_row(t.query(r), t.k, t.v, t.k_row, t.v_row, t.begin, t.limit(r), t.more_k, t.more_v, t.more_k_row,
-                                 t.more_v_row, t.more_end, size, scale);
+        const f32x4 v = slow_row(t.query(r), t.k, t.v, t.k_row, t.v_row, t.begin, t.limit(r), size, scale);
         for (int i = 0; i < 2; ++i) {
           const int d = 2 * lane + i;
           if (d >= size) continue;
@@ -628,8 +598,7 @@ struct Core {
           for (int g = 0; g < kAt; ++g) {
             if (!(bad >> (g * kLanes) & (kLanes == 64 ? ~0ull : (1ull << kLanes) - 1))) continue;
             const int row = r - lane / kLanes + g;
-            const f32x4 v = slow_row(t.query(row), t.k, t.v, t.k_row, t.v_row, t.begin, t.limit(row), t.more_k, t.more_v,
-                                     t.more_k_row, t.more_v_row, t.more_end, size, scale);
+            const f32x4 v = slow_row(t.query(row), t.k, t.v, t.k_row, t.v_row, t.begin, t.limit(row), size, scale);
             // Lane l holds channels 2 l, 2 l + 1.
             f32x4 w;
             for (int i = 0; i < 4; ++i) w[i] = __shfl(i & 1 ? v[1] : v[0], 2 * chunk + (i >> 1), 64);
@@ -739,7 +708,6 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void packed_kernel(fah_packed_atte
   t.head0 = p.row0 - token0 * group;
   t.first_limit = p.first_limit + token0;
   t.causal = true;
-  t.more_end = 0;
   t.begin = 0;
   t.end = p.keys;
   Sink<Q> sink{};
@@ -838,10 +806,8 @@ __global__ __launch_bounds__(kThreads) void packed_join_kernel(fah_packed_attent
 // How prefix_kernel's work is cut: prefix tiles of BM rows (a row is a sequence
 // and a head of the group) times shares of the prefix, then for every sequence
 // tiles of 32 heads times shares of its own rows.
-// `both`: few rows and keys; a sequence's tiles attend the prefix themselves.
 struct PrefixCut {
   int tiles, shares, own_tiles, own_shares;
-  bool both;
   int64_t prefix_items, own_items;
 };
 
@@ -862,7 +828,6 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_kernel(fah_prefix_attentio
   t.group = group;
   t.group_inverse = 1.0f / (float)group;
   t.causal = false;
-  t.more_end = 0;
   if (blockIdx.x < cut.prefix_items) {
     using C = Shared;
     const int head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
@@ -900,23 +865,9 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_kernel(fah_prefix_attentio
     t.v_row = (unsigned)a.value_row;
     t.head0 = tile * C::BM;
     t.rows = clamp_int(group - t.head0, 0, C::BM);
-    if (cut.both) {
-      t.more_k = t.k;
-      t.more_v = t.v;
-      t.more_k_row = t.k_row;
-      t.more_v_row = t.v_row;
-      t.more_end = length;
-      t.k = static_cast<const K*>(a.prefix_key) + head * a.prefix_key_head;
-      t.v = static_cast<const K*>(a.prefix_value) + head * a.prefix_value_head;
-      t.k_row = (unsigned)a.prefix_key_row;
-      t.v_row = (unsigned)a.prefix_value_row;
-      t.begin = 0;
-      t.end = a.prefix;
-    } else {
-      const int share = ((length + C::TR - 1) / C::TR + cut.own_shares - 1) / cut.own_shares * C::TR;
-      t.begin = share_at * share;
-      t.end = t.begin + share < length ? t.begin + share : length;
-    }
+    const int share = ((length + C::TR - 1) / C::TR + cut.own_shares - 1) / cut.own_shares * C::TR;
+    t.begin = share_at * share;
+    t.end = t.begin + share < length ? t.begin + share : length;
     t.first_limit = t.end;
     if (cut.prefix_items == 0 && cut.own_shares == 1) {
       sink.out = static_cast<Q*>(a.output) + s * a.output_sequence + (int64_t)head * group * a.output_head;
@@ -990,12 +941,10 @@ PrefixCut prefix_cut(const fah_prefix_attention& a, int* waves_rows) {
   const int64_t own = (int64_t)a.sequences * a.kv_heads * c.own_tiles;
   *waves_rows = rows <= 32 ? 1 : ceil_div(rows, 64) * a.kv_heads < 1024 ? 2 : 4;
   c.own_shares = (int)std::max<int64_t>(1, std::min<int64_t>(256 / own, ceil_div(longest, 256)));
-  c.both = own <= 256 && (int64_t)a.prefix + longest <= 1024;
-  if (c.both) c.own_shares = 1, *waves_rows = 1;
   c.tiles = (int)ceil_div(rows, 32 * *waves_rows);
   const int64_t fill = own * c.own_shares >= 1024 ? 128 : 256;
   c.shares = (int)std::max<int64_t>(1, std::min<int64_t>(fill / (c.tiles * a.kv_heads), ceil_div(a.prefix, 256)));
-  c.prefix_items = a.prefix && !c.both ? (int64_t)c.tiles * a.kv_heads * c.shares : 0;
+  c.prefix_items = a.prefix ? (int64_t)c.tiles * a.kv_heads * c.shares : 0;
   c.own_items = own * c.own_shares;
   return c;
 }
