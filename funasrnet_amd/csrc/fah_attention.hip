@@ -627,47 +627,74 @@ struct Core {
 
 // ---- Packed prompts ---------------------------------------------------------------
 
-// The place of a sequence's first tile of BM rows among all tiles: floor(first
-// row / BM) + its number. Sequences may so leave one tile each empty, and no sum
-// over the earlier ones is needed.
 struct PackedTile {
   int begin, row0, rows, key_begin, keys, first_limit;  // rows 0: none
 };
 
-// A wave finds the tile's sequence with 64 probes at a time; the last ones read
-// all that the tile needs, so that up to 64 sequences cost one round of loads.
-__device__ __forceinline__ PackedTile packed_tile(const fah_packed_attention& a, int slot, int group, int BM) {
+// Sums of the lanes up to this one, over a wave.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // from 1, 2, 4 and 8 lanes before, in rows of 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row 0's last lane to row 1, row 2's to row 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row 1's last lane to rows 2 and 3
+  return v;
+}
+
+// Tile `at`, counted from the last tile of BM rows of the last sequence. A wave
+// cuts the sequences into 64 parts, counts their tiles, and goes on in the part
+// that has the tile: one round for up to 64 sequences. What is behind the first
+// tile is none, so that workgroups without one come last.
+__device__ __forceinline__ PackedTile packed_tile(const fah_packed_attention& a, int at, int group, int BM) {
   const int lane = threadIdx.x & 63;
   const int* ko = a.key_offsets ? a.key_offsets : a.query_offsets;
   auto rows_at = [&](int s) { return clamp_int(a.query_offsets[s], 0, a.query_rows); };
   PackedTile p{};
-  int lo = 0, hi = a.sequences;
-  while (hi - lo > 64) {
-    const int step = (hi - lo + 63) / 64, probe = lo + lane * step;
-    const bool ok = probe < hi && rows_at(probe) * group / BM + probe <= slot;
-    const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(ok));
-    if (n == 0) return p;
-    lo += (n - 1) * step;
-    hi = lo + step < hi ? lo + step : hi;
+  int lo = 0, hi = a.sequences, target = -1;
+  for (bool first = true;; first = false) {
+    const int part = (hi - lo + 63) / 64;
+    int q0 = 0, q1 = 0, k0 = 0, k1 = 0, tiles = 0;
+    auto tiles_of = [&] { return q1 > q0 ? ((q1 - q0) * group + BM - 1) / BM : 0; };
+    if (part == 1) {
+      const int s = lo + lane < hi ? lo + lane : hi - 1;
+      q0 = rows_at(s);
+      q1 = rows_at(s + 1);
+      k0 = clamp_int(ko[s], 0, a.key_rows);
+      k1 = clamp_int(ko[s + 1], 0, a.key_rows);
+      tiles = lo + lane < hi ? tiles_of() : 0;
+    } else {
+      const int from = lo + lane * part < hi ? lo + lane * part : hi, to = from + part < hi ? from + part : hi;
+      for (int s = from; s < to; ++s) {
+        q0 = rows_at(s);
+        q1 = rows_at(s + 1);
+        tiles += tiles_of();
+      }
+    }
+    const int through = wave_scan(tiles);
+    if (first) target = __builtin_amdgcn_readlane(through, 63) - 1 - at;
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(through > target);
+    if (target < 0 || past == 0) return p;
+    const int l = __builtin_ctzll(past);
+    auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+    target -= of(through - tiles);
+    if (part == 1) {
+      p.begin = of(q0);
+      const int queries = of(q1) - p.begin;
+      p.key_begin = of(k0);
+      p.keys = of(k1) > p.key_begin ? of(k1) - p.key_begin : 0;
+      p.first_limit = p.keys - queries + 1;
+      p.row0 = target * BM;
+      p.rows = clamp_int(queries * group - p.row0, 0, BM);
+      return p;
+    }
+    lo += l * part;
+    hi = lo + part < hi ? lo + part : hi;
   }
-  const int s = lo + lane < hi ? lo + lane : hi - 1;
-  const int q0 = rows_at(s), q1 = rows_at(s + 1), k0 = clamp_int(ko[s], 0, a.key_rows), k1 = clamp_int(ko[s + 1], 0, a.key_rows);
-  const int tile = q0 * group / BM + s;
-  const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lo + lane < hi && tile <= slot));
-  if (n == 0) return p;
-  auto of = [&](int v) { return __builtin_amdgcn_readlane(v, n - 1); };
-  p.begin = of(q0);
-  const int queries = of(q1) > p.begin ? of(q1) - p.begin : 0;
-  p.key_begin = of(k0);
-  p.keys = of(k1) > p.key_begin ? of(k1) - p.key_begin : 0;
-  p.first_limit = p.keys - queries + 1;
-  p.row0 = (slot - of(tile)) * BM;
-  p.rows = clamp_int(queries * group - p.row0, 0, BM);
-  return p;
 }
 
-// How packed_kernel's work is cut: tiles (slots) of 32 `rows` rows, whose keys
-// are cut into shares of about `share`, at most `splits`.
+// How packed_kernel's work is cut: tiles of 32 `rows` rows, at most `slots`, whose
+// keys are cut into shares of about `share`, at most `splits`.
 struct PackedCut {
   int rows, splits, share;
   int64_t slots;
@@ -690,7 +717,7 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void packed_kernel(fah_packed_atte
   using C = Core<Q, K, D, WR, WK, NK>;
   __shared__ __align__(16) unsigned char lds[C::kLds];
   const int group = a.heads / a.kv_heads, head = blockIdx.x % a.kv_heads;
-  const int rest = blockIdx.x / a.kv_heads, split = rest / (int)cut.slots, slot = (int)cut.slots - 1 - rest % (int)cut.slots;
+  const int rest = blockIdx.x / a.kv_heads, split = rest / (int)cut.slots, slot = rest % (int)cut.slots;
   const PackedTile p = packed_tile(a, slot, group, C::BM);
   if (p.rows == 0) return;
   const int token0 = p.row0 / group;
