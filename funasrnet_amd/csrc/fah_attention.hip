@@ -952,7 +952,7 @@ PackedCut packed_cut(const fah_packed_attention& a) {
   const bool cached = (a.key_rows - a.query_rows) / a.sequences >= 1024;
   if ((int64_t)a.longest_query * group <= 32) c.rows = 1;
   else if (cached) c.rows = rows_each >= 192 && items(4) * keys / 1280 >= 256 ? 4 : rows_each > 32 ? 2 : 1;
-  else c.rows = items(2) < kFill / 2 ? 1 : items(4) < kFill ? 2 : 4;
+  else c.rows = items(4) >= kFill || (items(4) >= 64 && a.longest_key <= 2 * items(4)) ? 4 : items(2) < 448 ? 1 : 2;
   c.slots = rows / (32 * c.rows) + a.sequences;
   const int64_t n = items(c.rows);
   c.share = (int)std::min<int64_t>(std::max<int64_t>(512, n * keys / kFill), 1280);
@@ -984,7 +984,7 @@ hipError_t packed_launch(const fah_packed_attention& a, const PackedCut& c, hipS
   auto kernel = packed_kernel<Q, K, D, WR, WK, NK>;
   kernel<<<(unsigned)(c.slots * c.splits * a.kv_heads), C::kThreads, 0, s>>>(a, c);
   if (c.splits > 1) {
-    const dim3 grid((unsigned)(c.slots * a.kv_heads), C::BM / (kThreads / (D / 4)));
+    const dim3 grid((unsigned)(c.slots * a.kv_heads), (unsigned)ceil_div(C::BM, kThreads / (D / 4)));
     packed_join_kernel<Q, D, C::BM><<<grid, kThreads, 0, s>>>(a, c);
   }
   return hipGetLastError();
