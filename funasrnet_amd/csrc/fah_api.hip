@@ -2137,9 +2137,11 @@ void require_workspace(const void* p, int64_t have, int64_t need) {
           "the workspace needs " + std::to_string(need) + " bytes at a 16-byte boundary");
 }
 
-// Most elements between two key or value rows: the kernels' offsets within 16
-// rows are 32-bit byte offsets.
-constexpr int64_t kRowStride = 1 << 26;
+// Most elements between two key or value rows: the kernels' offsets within 32
+// rows are byte offsets below 2^31.
+constexpr int64_t kRowStride = 1 << 25;
+// Most keys: a tile past the last one still counts in 32 bits.
+constexpr int kMostKeys = INT32_MAX - 4096;
 
 // False: declined.
 bool check_packed(const fah_packed_attention& a) {
@@ -2148,8 +2150,9 @@ bool check_packed(const fah_packed_attention& a) {
   require(a.heads > 0 && a.kv_heads > 0 && a.head_size > 0 && a.heads % a.kv_heads == 0,
           "heads must be a multiple of the K/V heads");
   require(std::isfinite(a.scale) && a.scale > 0, "the attention scale must be above 0");
-  require((int64_t)a.query_rows * a.heads <= INT32_MAX / 2 && (int64_t)a.sequences * a.heads <= INT32_MAX / 256,
-          "too many query rows or sequences");
+  require((int64_t)a.query_rows * a.heads <= INT32_MAX / 2 && (int64_t)a.sequences * a.heads <= INT32_MAX / 256 &&
+              a.key_rows <= kMostKeys,
+          "too many query rows, sequences or keys");
   return fah::attention_supported(a.heads, a.kv_heads, a.head_size, a.query_type, a.cache_type) &&
          strides16(a.query_type, {a.query_row, a.query_head, a.output_row, a.output_head}) &&
          strides16(a.cache_type, {a.key_row, a.key_head, a.value_row, a.value_head}) &&
@@ -2161,7 +2164,8 @@ bool check_prefix(const fah_prefix_attention& a) {
   require(a.heads > 0 && a.kv_heads > 0 && a.head_size > 0 && a.heads % a.kv_heads == 0,
           "heads must be a multiple of the K/V heads");
   require(std::isfinite(a.scale) && a.scale > 0, "the attention scale must be above 0");
-  require((int64_t)a.sequences * a.heads <= INT32_MAX / 256, "too many sequences");
+  require((int64_t)a.sequences * a.heads <= INT32_MAX / 256 && a.prefix <= kMostKeys && a.capacity <= kMostKeys,
+          "too many sequences or keys");
   return fah::attention_supported(a.heads, a.kv_heads, a.head_size, a.query_type, a.cache_type) &&
          strides16(a.query_type, {a.query_sequence, a.query_head, a.output_sequence, a.output_head}) &&
          strides16(a.cache_type, {a.prefix_key_row, a.prefix_key_head, a.prefix_value_row, a.prefix_value_head,

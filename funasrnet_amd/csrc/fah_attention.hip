@@ -1,6 +1,35 @@
 // Attention of the serving operators: packed causal prompts and single tokens
 // behind a shared prefix, grouped heads (fah_packed_attention and
 // fah_prefix_attention of the C ABI).
+//
+// Per row, o = sum_j 2^(c s_j - r) v_j / sum_j 2^(c s_j - r) with s = q k and
+// c = scale log2(e), in one pass over the keys: r is a reference that follows
+// the largest score seen, and sums made with an earlier one are scaled when it
+// moves. A row is a (token, query head of the K/V head's group) pair, so a tile
+// of K and V serves all heads of a group.
+//
+// Layout. A wave has 32 rows. It forms S^T = K Q^T with 32 x 32 x 16 matrix
+// instructions (keys x rows), whose result leaves each lane with 16 keys of one
+// row: the softmax is per lane but for one exchange between the wave's halves,
+// and the weights are, as they stand, the B operand of O^T = V^T P^T, whose sums
+// again belong to the lane's row. Which key a B element is, is free as long as
+// V^T's A operand names the same: it is read from the row-major tile by the
+// transposing LDS read, four keys by 16 channels at a time. K and V tiles come
+// by direct loads into LDS, 16 bytes a lane, in a swizzled order (0 bank
+// conflicts counted).
+//
+// Rounding. Scores, references, totals and sums are fp32. Weights are rounded
+// once to the values' type, as the matrix instructions take them (totals are of
+// the unrounded ones); it is the only rounding that fp32 arithmetic on the same
+// inputs has not, and adds to the error what rounding the output does: measured
+// 2.3e-3 of the result in bf16 against 1.7e-3. fp32 queries, and the weights of
+// their rows, are split into two fp16 parts and take two products each: 3e-7.
+//
+// What bounds it: long prompts the matrix instructions and the card's power
+// (8192 rows of 32/8 heads in bf16: 525 us, 1.05 PFLOP/s, matrix units 52% busy
+// at 1.9 GHz; a library product of 8192^3 reaches 1.21); own cache rows of a
+// large batch the memory (256 sequences: 128 us, 5.2 TB/s); everything small the
+// chain offsets, queries and first tile, one pass, epilogue: 5 to 6 us.
 #include "fah_device.h"
 #include "fah_internal.h"
 
@@ -60,9 +89,8 @@ struct Task {
   int begin, end;            // keys
   int first_limit;           // token 0 sees the keys below this; per token one more if causal
   bool causal;
-  // Row r's token and head. (r + head0 is below 2^20: the product is within a
-  // quarter of the exact quotient, which is at least half a step from a whole
-  // number's edge.)
+  // Row r's token and head. r + head0 is below 65536 + 128: the product's error,
+  // 2^-22 of it, is far below the half step that it is from a whole number.
   __device__ __forceinline__ int token(int r) const { return (int)((float)(r + head0) * group_inverse + 0.5f * group_inverse); }
   __device__ __forceinline__ int head(int r) const { return r + head0 - token(r) * group; }
   __device__ __forceinline__ int limit(int r) const {
@@ -216,7 +244,11 @@ __device__ __forceinline__ unsigned pack2(float a, float b) {
 }
 
 // The workgroup's waves as WR groups of 32 rows times WK shares of each key
-// tile; a wave takes NK keys of a tile.
+// tile; a wave takes NK keys of a tile. Used as 4 x 1 (64 keys a wave), 2 x 2 and
+// 1 x 4 (32 keys): the first loads the fewest bytes a product, the last gives few
+// rows the most waves. Eight waves (2 x 4, 4 x 2, 1 x 8) were slower everywhere,
+// and so were scores formed a tile ahead of the weights (256 registers do not
+// hold both: 8192 rows 675 us).
 template <typename Q, typename K, int D, int WR, int WK, int NK>
 struct Core {
   static constexpr int kWaves = WR * WK, kThreads = 64 * kWaves, BM = 32 * WR, TR = WK * NK;
@@ -417,8 +449,9 @@ struct Core {
       const unsigned char* vt = lds + shift + kTileBytes;
 #pragma unroll
       for (int step = 0; step < NK / 16; ++step) {
-        // The B operand of 16 keys: a lane's eight weights as they are; the
-        // values are read in the same key order.
+        // The B operand of 16 keys: a lane's eight weights as they are, rounded
+        // to the values' type (see the top); the values are read in the same key
+        // order.
         uint4 hi, lo;
         unsigned* ph = reinterpret_cast<unsigned*>(&hi);
         unsigned* pl = reinterpret_cast<unsigned*>(&lo);
@@ -940,10 +973,22 @@ __global__ __launch_bounds__(kThreads) void prefix_join_kernel(fah_prefix_attent
 
 // ---- Launch rules -------------------------------------------------------------------
 
-constexpr int kFill = 512;  // workgroups that fill the chip
+constexpr int kFill = 512;  // workgroups that fill the chip: two a CU
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Rows of a tile. 128 where that fills the chip; and with fewer items where the
+// sequences are short, because what a workgroup spends around its passes (5 us)
+// then counts more than the passes (30 x 100 rows: 17.7 us, 28 with 64 rows;
+// 4 x 819: 28.6 against 32; but one of 3200: 69 against 62). 32 where 64-row
+// tiles leave CUs without work (750 rows: 15.5 us, 21.5 with 64 rows) or a
+// sequence has no more rows. Behind long caches the same by the work that the
+// keys' shares make of the items.
+//
+// Shares of the keys only behind long caches: the joined rows pass through
+// memory and a second launch (six resumed prompts 50 us, 60 at best without;
+// one token behind 5000 keys 15.5 against 49; a prompt alone of 3200 rows 74
+// against 62).
 PackedCut packed_cut(const fah_packed_attention& a) {
   const int group = a.heads / a.kv_heads;
   const int64_t rows = (int64_t)a.query_rows * group, keys = a.key_rows / a.sequences, rows_each = rows / a.sequences;
@@ -960,6 +1005,14 @@ PackedCut packed_cut(const fah_packed_attention& a) {
   return c;
 }
 
+// Few and long shares of the prefix: each costs its rows' partial sums twice
+// through memory. 256 items, or 128 where the sequences' own rows fill the chip
+// beside them, of 256 to 4096 keys (61 sequences behind 8191 keys: 26 us with 256
+// items, 34 with 128, 29 to 45 with 512; 256 behind 4096, own rows 128 to 133 us
+// with 64 or 128 items, 142 with 256; 256 behind 8000, fp32: 84 us with shares of
+// 4000 keys, 133 with one). 64 rows a tile until 1024 of them (256 sequences of
+// 8 heads a group: 65 us, 86 with 128 rows; 1024 sequences 185 against 173); 32
+// for no more rows.
 PrefixCut prefix_cut(const fah_prefix_attention& a, int* waves_rows) {
   const int group = a.heads / a.kv_heads, longest = std::min(a.longest, a.capacity);
   const int64_t rows = (int64_t)a.sequences * group;
@@ -970,7 +1023,7 @@ PrefixCut prefix_cut(const fah_prefix_attention& a, int* waves_rows) {
   c.own_shares = (int)std::max<int64_t>(1, std::min<int64_t>(256 / own, ceil_div(longest, 256)));
   c.tiles = (int)ceil_div(rows, 32 * *waves_rows);
   const int64_t fill = own * c.own_shares >= 1024 ? 128 : 256;
-  c.shares = (int)std::max<int64_t>(1, std::min<int64_t>(fill / (c.tiles * a.kv_heads), ceil_div(a.prefix, 256)));
+  c.shares = (int)std::max<int64_t>({1, ceil_div(a.prefix, 4096), std::min<int64_t>(fill / (c.tiles * a.kv_heads), ceil_div(a.prefix, 256))});
   c.prefix_items = a.prefix ? (int64_t)c.tiles * a.kv_heads * c.shares : 0;
   c.own_items = own * c.own_shares;
   return c;
@@ -1018,7 +1071,7 @@ hipError_t prefix_typed(const fah_prefix_attention& a, hipStream_t s) {
 }  // namespace
 
 bool attention_supported(int heads, int kv_heads, int head_size, int query_type, int cache_type) {
-  return heads % kv_heads == 0 && head_size % 8 == 0 && head_size <= 128 &&
+  return heads <= 65536 && head_size % 8 == 0 && head_size <= 128 &&
          ((query_type == FAH_TYPE_F32 && cache_type == FAH_TYPE_F16) ||
           (query_type == FAH_TYPE_F16 && cache_type == FAH_TYPE_F16) ||
           (query_type == FAH_TYPE_BF16 && cache_type == FAH_TYPE_BF16));

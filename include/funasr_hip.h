@@ -305,9 +305,9 @@ typedef struct fah_packed_attention {
     int64_t workspace_bytes;
 } fah_packed_attention;
 
-/* Declines head sizes that are no multiple of 8 or above 128, other pairs of
- * types, rows that do not start on 16 bytes (addresses and strides), and key
- * or value rows more than 2^26 elements apart. */
+/* Declines head sizes that are no multiple of 8 or above 128, more than 65536
+ * heads, other pairs of types, rows that do not start on 16 bytes (addresses and
+ * strides), and key or value rows more than 2^25 elements apart. */
 int fah_attention_packed_device(fah_context* context, const fah_packed_attention* call);
 int fah_attention_packed_workspace(const fah_packed_attention* call, int64_t* bytes);
 

@@ -66,7 +66,8 @@ def test_null_arguments(kind):
     ("packed", dict(longest_query=-1)), ("packed", dict(longest_key=-1)), ("packed", dict(heads=0)),
     ("packed", dict(kv_heads=0)), ("packed", dict(kv_heads=3)), ("packed", dict(head_size=0)), ("packed", dict(scale=0.0)),
     ("packed", dict(scale=-1.0)), ("packed", dict(scale=float("nan"))), ("packed", dict(scale=float("inf"))),
-    ("packed", dict(query_rows=2**31 - 1)), ("packed", dict(sequences=2**31 - 1)),
+    ("packed", dict(query_rows=2**31 - 1)), ("packed", dict(sequences=2**31 - 1)), ("packed", dict(key_rows=2**31 - 1)),
+    ("prefix", dict(prefix=2**31 - 1)), ("prefix", dict(capacity=2**31 - 1)),
     ("prefix", dict(sequences=-1)), ("prefix", dict(prefix=-1)), ("prefix", dict(capacity=-1)), ("prefix", dict(longest=-1)),
     ("prefix", dict(heads=15)), ("prefix", dict(kv_heads=-8)), ("prefix", dict(scale=0.0)),
     ("prefix", dict(sequences=2**31 - 1)),
@@ -83,7 +84,8 @@ def test_invalid_sizes_are_errors(kind, changes):
     ("packed", dict(head_size=12)), ("packed", dict(head_size=136)), ("packed", dict(query_type=hip.TYPE_F32, cache_type=0)),
     ("packed", dict(query_type=hip.TYPE_F16, cache_type=hip.TYPE_BF16)), ("packed", dict(query_type=7)),
     ("packed", dict(query_row=2046)), ("packed", dict(output_head=130)), ("packed", dict(key_row=1028)),
-    ("packed", dict(value_head=-128)),
+    ("packed", dict(value_head=-128)), ("packed", dict(key_row=(1 << 25) + 8)), ("packed", dict(heads=65544, kv_heads=8)),
+    ("prefix", dict(value_row=(1 << 25) + 8)),
     ("prefix", dict(head_size=100)), ("prefix", dict(cache_type=hip.TYPE_BF16)), ("prefix", dict(prefix_key_row=132)),
     ("prefix", dict(key_sequence=(1 << 20) + 4)), ("prefix", dict(query_head=2)), ("prefix", dict(output_sequence=-2048)),
     ("logits", dict(type=3)), ("logits", dict(type=-1)),
