@@ -47,7 +47,6 @@ using s16x4 = __attribute__((ext_vector_type(4))) short;
 using s16x8 = __attribute__((ext_vector_type(8))) short;
 using LdsTr = s16x4 __attribute__((address_space(3))) *;
 using LdsFrag = s16x8 __attribute__((address_space(3))) *;
-using LdsDma = __attribute__((address_space(3))) void*;
 
 constexpr int kThreads = 256;
 constexpr float kInf = __builtin_inff();
@@ -347,8 +346,10 @@ struct Core {
         for (int w = 0; w < kWaves; ++w) most = fmaxf(most, marks[w * 32 + col]);
         lds_barrier();
       }
+      // With an infinity in it the row's scores are infinite or NaN whatever the
+      // second parts hold: they are 0, for infinity - infinity is not.
       const int e = (int)(f2u(most) >> 23) - 127;
-      const int up = e == 128 ? 0 : clamp_int(13 - e, -114, 126);
+      const int up = clamp_int(13 - e, -114, 126);
       const float lift = u2f((unsigned)(up + 127) << 23);
 #pragma unroll
       for (int s = 0; s < kMine; ++s) {
@@ -357,7 +358,7 @@ struct Core {
         for (int j = 0; j < 8; ++j) {
           const float v = raw[s][j >> 2][j & 3] * lift;
           hi[j] = (_Float16)v;
-          lo[j] = (_Float16)(v - (float)hi[j]);
+          lo[j] = (_Float16)(e == 128 ? 0.0f : v - (float)hi[j]);
         }
         part[0][s] = __builtin_bit_cast(s16x8, hi);
         part[kSplit ? 1 : 0][s] = __builtin_bit_cast(s16x8, lo);

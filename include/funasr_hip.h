@@ -270,8 +270,9 @@ int fah_q8_block_dots_device(fah_context* context, const int8_t* q, const fah_we
  * may be captured into graphs. What they need beyond their outputs is the
  * caller's `workspace`: at least the bytes that the *_workspace call of the
  * same descriptor gives (it needs no device and reads nothing through the
- * pointers), 16-byte aligned, its contents free before and after. Calls that may run at the same time, such as two
- * graphs replayed on different streams, need workspaces of their own.
+ * pointers), 16-byte aligned, its contents free before and after. Calls that
+ * may run at the same time, such as two graphs replayed on different streams,
+ * need workspaces of their own.
  * No output may overlap an input or the workspace unless its comment says so. */
 
 /* Element types. */

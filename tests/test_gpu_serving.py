@@ -209,6 +209,22 @@ def test_packed_row_of_minus_infinity_scores(backend):
         assert np.all(np.abs(got[3:, h] - out) <= attention_bound(out, weight, dots, 37, 64, "f16"))
 
 
+@pytest.mark.parametrize("rows,heads,kv_heads", [(40, 2, 2), (300, 16, 1)])
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(t))
+def test_packed_infinite_queries(backend, types, rows, heads, kv_heads):
+    """-infinity against keys above 0: every score is -infinity, the row zeros; other rows as ever."""
+    q, k, v = packed_inputs(10, [rows], [rows], heads, kv_heads, 128, types)
+    k[:, :, 5] = store(np.abs(load(k[:, :, 5], types[1])) + 0.125, types[1])
+    plain = load(run_packed(backend, q, k, v, offsets([rows]), None, types), types[0])
+    q[3::7, :, 5] = store(np.full(q[3::7, :, 5].shape, -np.inf), types[0])
+    q[5::7, :, 5] = store(np.full(q[5::7, :, 5].shape, np.inf), types[0])  # infinity - infinity
+    got = load(run_packed(backend, q, k, v, offsets([rows]), None, types), types[0])
+    assert np.all(got[3::7] == 0)
+    assert np.all(np.isnan(got[5::7]))
+    others = np.isin(np.arange(rows) % 7, [3, 5], invert=True)
+    assert np.array_equal(got[others], plain[others])
+
+
 @pytest.mark.parametrize("magnitude", [1e-30, 1e-6, 1e4, 1e30])
 def test_packed_fp32_queries_of_any_size(backend, magnitude):
     types = ("f32", "f16")
