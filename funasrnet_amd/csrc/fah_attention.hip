@@ -676,11 +676,26 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
+__device__ __forceinline__ int wave_sum(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+// The largest of the lanes' values, none below 0.
+__device__ __forceinline__ int wave_max(int v) {
+  for (int x = 32; x >= 1; x >>= 1) {
+    const int other = __shfl_xor(v, x, 64);
+    v = other > v ? other : v;
+  }
+  return (int)uniform((unsigned)v);
+}
+
 // Tile `at`, counted from the last tile of BM rows of the last sequence. A wave
 // cuts the sequences into 64 parts, counts their tiles, and goes on in the part
 // that has the tile: one round for up to 64 sequences. What is behind the first
 // tile is none, so that workgroups without one come last.
-__device__ __forceinline__ PackedTile packed_tile(const fah_packed_attention& a, int at, int group, int BM) {
+// levels: 2 to 64 sequences' tiles are counted level by level from the highest,
+// all sequences' third tiles before their second ones: a tile's passes grow with
+// its place, and the longest must not start last (24 prompts 27 us, 33 in the
+// other order; but six behind caches 56 against 50, whose tiles then share no
+// keys with those beside them).
+__device__ __forceinline__ PackedTile packed_tile(const fah_packed_attention& a, int at, int group, int BM, bool levels) {
   const int lane = threadIdx.x & 63;
   const int* ko = a.key_offsets ? a.key_offsets : a.query_offsets;
   auto rows_at = [&](int s) { return clamp_int(a.query_offsets[s], 0, a.query_rows); };
@@ -690,6 +705,18 @@ __device__ __forceinline__ PackedTile packed_tile(const fah_packed_attention& a,
     const int part = (hi - lo + 63) / 64;
     int q0 = 0, q1 = 0, k0 = 0, k1 = 0, tiles = 0;
     auto tiles_of = [&] { return q1 > q0 ? ((q1 - q0) * group + BM - 1) / BM : 0; };
+    // Tile n of lane l's sequence.
+    auto tile = [&](int l, int n) {
+      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+      p.begin = of(q0);
+      const int queries = of(q1) - p.begin;
+      p.key_begin = of(k0);
+      p.keys = of(k1) > p.key_begin ? of(k1) - p.key_begin : 0;
+      p.first_limit = p.keys - queries + 1;
+      p.row0 = n * BM;
+      p.rows = clamp_int(queries * group - p.row0, 0, BM);
+      return p;
+    };
     if (part == 1) {
       const int s = lo + lane < hi ? lo + lane : hi - 1;
       q0 = rows_at(s);
@@ -705,23 +732,25 @@ __device__ __forceinline__ PackedTile packed_tile(const fah_packed_attention& a,
         tiles += tiles_of();
       }
     }
+    if (levels && part == 1) {
+      int low = 0, high = wave_max(tiles), count = wave_sum(tiles), above = 0;
+      if (at >= count) return p;
+      while (high - low > 1) {  // `low`: more than `at` tiles are there or higher; `high`: not
+        const int mid = (low + high) / 2, n = wave_sum(tiles > mid ? tiles - mid : 0);
+        if (n > at) low = mid;
+        else high = mid, above = n;
+      }
+      const unsigned long long there = __builtin_amdgcn_ballot_w64(tiles > low);
+      const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(there >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)there, 0));
+      return tile(__builtin_ctzll(__builtin_amdgcn_ballot_w64(tiles > low && before == at - above)), low);
+    }
     const int through = wave_scan(tiles);
     if (first) target = __builtin_amdgcn_readlane(through, 63) - 1 - at;
     const unsigned long long past = __builtin_amdgcn_ballot_w64(through > target);
     if (target < 0 || past == 0) return p;
     const int l = __builtin_ctzll(past);
-    auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-    target -= of(through - tiles);
-    if (part == 1) {
-      p.begin = of(q0);
-      const int queries = of(q1) - p.begin;
-      p.key_begin = of(k0);
-      p.keys = of(k1) > p.key_begin ? of(k1) - p.key_begin : 0;
-      p.first_limit = p.keys - queries + 1;
-      p.row0 = target * BM;
-      p.rows = clamp_int(queries * group - p.row0, 0, BM);
-      return p;
-    }
+    target -= __builtin_amdgcn_readlane(through - tiles, l);
+    if (part == 1) return tile(l, target);
     lo += l * part;
     hi = lo + part < hi ? lo + part : hi;
   }
@@ -752,7 +781,7 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void packed_kernel(fah_packed_atte
   __shared__ __align__(16) unsigned char lds[C::kLds];
   const int group = a.heads / a.kv_heads, head = blockIdx.x % a.kv_heads;
   const int rest = blockIdx.x / a.kv_heads, split = rest / (int)cut.slots, slot = rest % (int)cut.slots;
-  const PackedTile p = packed_tile(a, slot, group, C::BM);
+  const PackedTile p = packed_tile(a, slot, group, C::BM, cut.splits == 1 && a.sequences > 1 && a.sequences <= 64);
   if (p.rows == 0) return;
   const int token0 = p.row0 / group;
   Task<Q, K> t;
@@ -802,6 +831,13 @@ struct Joined {
     const int lane = threadIdx.x % kLanes;
     for (int first = 0; first < count; first += kLanes) {
       const int n = count - first < kLanes ? count - first : kLanes;
+      // Eight rows at a time, the first ones requested with the marks.
+      f32x4 v[8];
+      auto request = [&](int i0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const f32x4*>(at(first + (i0 + i < n ? i0 + i : n - 1)));
+      };
+      request(0);
       float m = -kInf, w = 0.0f;
       if (lane < n) {
         const float2 mark = *reinterpret_cast<const float2*>(marks(first + lane));
@@ -817,11 +853,8 @@ struct Joined {
       for (int x = kLanes / 2; x >= 1; x >>= 1) sum += __shfl_xor(sum, x, kLanes);
       total = total * keep + sum;
       o *= keep;
-      // Eight at a time, all requested before the first is used.
       for (int i0 = 0; i0 < n; i0 += 8) {
-        f32x4 v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const f32x4*>(at(first + (i0 + i < n ? i0 + i : n - 1)));
+        if (i0 > 0) request(i0);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float wi = __shfl(weight, (i0 + i) % kLanes, kLanes);  // 0 from n on
@@ -846,7 +879,7 @@ struct Joined {
 template <typename Q, int D, int BM>
 __global__ __launch_bounds__(kThreads) void packed_join_kernel(fah_packed_attention a, PackedCut cut) {
   const int group = a.heads / a.kv_heads, head = blockIdx.x % a.kv_heads, slot = blockIdx.x / a.kv_heads;
-  const PackedTile p = packed_tile(a, slot, group, BM);
+  const PackedTile p = packed_tile(a, slot, group, BM, false);
   constexpr int kLanes = D / 4;
   const int chunk = threadIdx.x % kLanes, r = blockIdx.y * (kThreads / kLanes) + threadIdx.x / kLanes;
   if (r >= p.rows) return;
