@@ -1013,8 +1013,8 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Rows of a tile. 128 where that fills the chip; and with fewer items where the
 // sequences are short, because what a workgroup spends around its passes (5 us)
-// then counts more than the passes (30 x 100 rows: 17.7 us, 28 with 64 rows;
-// 4 x 819: 28.6 against 32; but one of 3200: 69 against 62). 32 where 64-row
+// then counts more than the passes (30 x 100 rows, 16/8 heads: 14.2 us, 20.7 with
+// 64 rows; 4 x 819: 26.1 against 31.4; but one of 3200: 69 against 62). 32 where 64-row
 // tiles leave CUs without work (750 rows: 15.5 us, 21.5 with 64 rows) or a
 // sequence has no more rows. Behind long caches the same by the work that the
 // keys' shares make of the items.

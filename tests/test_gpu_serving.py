@@ -578,6 +578,28 @@ def test_choice(backend, kind, rows, vocab, history, biases, masks, pad):
     assert np.array_equal(got.view(np.uint8), alone.view(np.uint8))
 
 
+@pytest.mark.parametrize("kind,rows", [("f32", 120), ("f32", 330), ("f32", 430), ("bf16", 250), ("bf16", 870)])
+def test_choice_of_large_batches(backend, kind, rows):
+    """Workgroups that take several chunks of a row, lists that name few or nearly all tokens of a chunk."""
+    vocab, history, biases = 20011, 3500, 700
+    v = choice_inputs(rows, rows, vocab, history, biases, 3, kind)
+    rng = np.random.default_rng(rows)
+    for r in range(rows):
+        if r % 3 == 0:    # few
+            v["counts"][r], v["bias_counts"][r] = 40, 9
+        elif r % 3 == 1:  # every token of a range, in any order
+            start = int(rng.integers(0, vocab - history))
+            v["history"][r] = start + rng.permutation(history)
+            v["bias_tokens"][r] = start + rng.permutation(biases) - 50
+            v["counts"][r], v["bias_counts"][r] = history, biases
+        else:             # one token
+            v["history"][r] = r
+    got, picked = run_choice(backend, v, kind, pad=5)
+    for at in (slice(0, 40), slice(rows // 2, rows // 2 + 9), slice(rows - 9, rows)):
+        some = {n: a if n == "masks" else a[at] for n, a in v.items()}
+        check_choice(got[at], picked[at], some, kind)
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 def test_choice_of_unusual_values(backend, kind):
     v = choice_inputs(3, 6, 700, 30, 5, 0, kind)
