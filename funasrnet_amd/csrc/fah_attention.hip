@@ -28,7 +28,7 @@
 // What bounds it: long prompts the matrix instructions and the card's power
 // (8192 rows of 32/8 heads in bf16: 525 us, 1.05 PFLOP/s, matrix units 52% busy
 // at 1.9 GHz; a library product of 8192^3 reaches 1.21); own cache rows of a
-// large batch the memory (256 sequences: 128 us, 5.2 TB/s); everything small the
+// large batch the memory (256 sequences: 121 us, 5.5 TB/s); everything small the
 // chain offsets, queries and first tile, one pass, epilogue: 5 to 6 us.
 #include "fah_device.h"
 #include "fah_internal.h"
@@ -131,12 +131,21 @@ __device__ __forceinline__ const void* uniform(const void* p) {
 // 16 bytes a lane from base + offset to LDS at `to` + 16 lane. Inline, because
 // the compiler would wait for a load into LDS before any read of LDS: the
 // tiles' reads are ordered by wait_loads and a barrier instead. (It has no
-// register that it writes; a load into M0's place needs one wait state.)
+// register that it writes; a load into M0's place needs one wait state.) ONCE:
+// past the caches.
+template <bool ONCE>
 __device__ __forceinline__ void load_lds(const void* base, unsigned offset, unsigned to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(uniform(to)), "v"(offset), "s"(uniform(base)) : "memory");
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(uniform(to)), "v"(offset), "s"(uniform(base)) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(uniform(to)), "v"(offset), "s"(uniform(base)) : "memory");
 }
+template <bool ONCE>
 __device__ __forceinline__ void load_lds(const void* from, unsigned to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(uniform(to)), "v"(from) : "memory");
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(uniform(to)), "v"(from) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(uniform(to)), "v"(from) : "memory");
 }
 // Every load of this wave is done (vmcnt 0, nothing else waited for). A barrier
 // follows: reads of LDS may move up to it but not before it.
@@ -157,7 +166,7 @@ __device__ __forceinline__ unsigned lds_address(const void* p) {
 // Loads tiles of ROWS keys or values by the waves w of W, kRowsLoad rows a load.
 // A lane's place in the source repeats, but for the base, after the rows whose
 // swizzles differ: its offsets are kept, and the base moves in scalar registers.
-template <typename K, int D, int ROWS, int W, bool VALUES>
+template <typename K, int D, int ROWS, int W, bool VALUES, bool ONCE>
 struct Loader {
   using T = Tile<D>;
   static constexpr int kLoads = ROWS / T::kRowsLoad / W, kStep = W * T::kRowsLoad;
@@ -186,7 +195,7 @@ struct Loader {
       const K* at = base + (int64_t)first * stride;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i)
-        load_lds(at + (int64_t)(i / kKinds * kKinds * kStep) * stride, offset[i % kKinds], to + shift + i * W * 1024);
+        load_lds<ONCE>(at + (int64_t)(i / kKinds * kKinds * kStep) * stride, offset[i % kKinds], to + shift + i * W * 1024);
     } else {
       // Rows past `last` repeat it (their scores are masked); places behind
       // head_size stay as they are (zero).
@@ -194,7 +203,7 @@ struct Loader {
       for (int i = 0; i < kLoads; ++i) {
         const int r = row0 + i * kStep + (threadIdx.x & 63) / T::kChunks;
         const int row = first + r < last ? first + r : last;
-        if (chunk(r) * 8 < size) load_lds(base + (int64_t)row * stride + chunk(r) * 8, to + shift + i * W * 1024);
+        if (chunk(r) * 8 < size) load_lds<ONCE>(base + (int64_t)row * stride + chunk(r) * 8, to + shift + i * W * 1024);
       }
     }
   }
@@ -248,7 +257,7 @@ __device__ __forceinline__ unsigned pack2(float a, float b) {
 // rows the most waves. Eight waves (2 x 4, 4 x 2, 1 x 8) were slower everywhere,
 // and so were scores formed a tile ahead of the weights (256 registers do not
 // hold both: 8192 rows 675 us).
-template <typename Q, typename K, int D, int WR, int WK, int NK>
+template <typename Q, typename K, int D, int WR, int WK, int NK, bool ONCE = false>
 struct Core {
   static constexpr int kWaves = WR * WK, kThreads = 64 * kWaves, BM = 32 * WR, TR = WK * NK;
   static constexpr int kTileBytes = TR * 2 * D;        // keys, or values
@@ -285,8 +294,8 @@ struct Core {
     }
     constexpr int kOwn = WR == 1 ? NK : TR, kLoaders = WR == 1 ? 1 : kWaves;
     const int own = WR == 1 ? wave * NK : 0, loader = WR == 1 ? 0 : wave;
-    using KeyLoader = Loader<K, D, kOwn, kLoaders, false>;
-    using ValueLoader = Loader<K, D, kOwn, kLoaders, true>;
+    using KeyLoader = Loader<K, D, kOwn, kLoaders, false, ONCE>;
+    using ValueLoader = Loader<K, D, kOwn, kLoaders, true, ONCE>;
     const KeyLoader key_loader(lds + own * T::kRowBytes, t.k_row, loader);
     const ValueLoader value_loader(lds + kTileBytes + own * T::kRowBytes, t.v_row, loader);
     // The wave's first key, and the end of those that its rows see.
@@ -907,10 +916,11 @@ struct PrefixCut {
 
 // Partial rows: [K/V head][share][sequences * group][D + 2] of the prefix, then
 // [sequence][K/V head][own share][group][D + 2]; a row's sums, then its marks.
-template <typename Q, typename K, int D, int WR, int WK, int NK>
+// ONCE: own rows pass the caches by.
+template <typename Q, typename K, int D, int WR, int WK, int NK, bool ONCE>
 __global__ __launch_bounds__(kThreads, 2) void prefix_kernel(fah_prefix_attention a, PrefixCut cut) {
   using Shared = Core<Q, K, D, WR, WK, NK>;
-  using Own = Core<Q, K, D, 1, 4, 32>;
+  using Own = Core<Q, K, D, 1, 4, 32, ONCE>;
   static_assert(Shared::kThreads == kThreads && Own::kThreads == kThreads);
   __shared__ __align__(16) unsigned char lds[std::max(Shared::kLds, Own::kLds)];
   const int group = a.heads / a.kv_heads;
@@ -1042,8 +1052,8 @@ PackedCut packed_cut(const fah_packed_attention& a) {
 // Few and long shares of the prefix: each costs its rows' partial sums twice
 // through memory. 256 items, or 128 where the sequences' own rows fill the chip
 // beside them, of 256 to 4096 keys (61 sequences behind 8191 keys: 26 us with 256
-// items, 34 with 128, 29 to 45 with 512; 256 behind 4096, own rows 128 to 133 us
-// with 64 or 128 items, 142 with 256; 256 behind 8000, fp32: 84 us with shares of
+// items, 34 with 128, 29 to 45 with 512; 256 behind 4096, own rows through the
+// caches, 128 to 133 us with 64 or 128 items, 142 with 256; 256 behind 8000, fp32: 84 us with shares of
 // 4000 keys, 133 with one). 64 rows a tile until 1024 of them (256 sequences of
 // 8 heads a group: 65 us, 86 with 128 rows; 1024 sequences 185 against 173); 32
 // for no more rows.
@@ -1085,9 +1095,9 @@ hipError_t packed_typed(const fah_packed_attention& a, hipStream_t s) {
   return packed_launch<Q, K, D, 4, 1, 64>(a, c, s);
 }
 
-template <typename Q, typename K, int D, int WR, int WK, int NK>
+template <typename Q, typename K, int D, int WR, int WK, int NK, bool ONCE>
 hipError_t prefix_launch(const fah_prefix_attention& a, const PrefixCut& c, hipStream_t s) {
-  prefix_kernel<Q, K, D, WR, WK, NK><<<(unsigned)(c.prefix_items + c.own_items), kThreads, 0, s>>>(a, c);
+  prefix_kernel<Q, K, D, WR, WK, NK, ONCE><<<(unsigned)(c.prefix_items + c.own_items), kThreads, 0, s>>>(a, c);
   if (c.prefix_items || c.own_shares > 1)
     prefix_join_kernel<Q, D><<<(unsigned)ceil_div((int64_t)a.sequences * a.heads, kThreads / (D / 4)), kThreads, 0, s>>>(a, c);
   return hipGetLastError();
@@ -1097,9 +1107,13 @@ template <typename Q, typename K, int D>
 hipError_t prefix_typed(const fah_prefix_attention& a, hipStream_t s) {
   int waves_rows;
   const PrefixCut c = prefix_cut(a, &waves_rows);
-  if (waves_rows == 1) return prefix_launch<Q, K, D, 1, 4, 32>(a, c, s);
-  if (waves_rows == 2) return prefix_launch<Q, K, D, 2, 2, 32>(a, c, s);
-  return prefix_launch<Q, K, D, 4, 1, 64>(a, c, s);
+  // Own rows are read once a call, and past the caches where these (256 MB)
+  // could not hold them to the next call (256 sequences of 800 rows on average:
+  // 121 us, 133 through the caches; 61 of 350: 27.8 against 26.2).
+  const bool once = (int64_t)a.sequences * std::min(a.longest, a.capacity) * a.kv_heads * a.head_size * 4 > 256 << 20;
+  if (waves_rows == 1) return prefix_launch<Q, K, D, 1, 4, 32, false>(a, c, s);
+  if (waves_rows == 2) return once ? prefix_launch<Q, K, D, 2, 2, 32, true>(a, c, s) : prefix_launch<Q, K, D, 2, 2, 32, false>(a, c, s);
+  return once ? prefix_launch<Q, K, D, 4, 1, 64, true>(a, c, s) : prefix_launch<Q, K, D, 4, 1, 64, false>(a, c, s);
 }
 
 }  // namespace

@@ -25,6 +25,15 @@ struct alignas(16) Vec {
   T v[kCount];
 };
 
+// 16 bytes past the caches: adjusted logits are not read again here, and would
+// push the rows to come out of them (256 rows of 151936 in bf16: 33.4 us,
+// 47.5 with plain stores; with loads past them as well 39).
+template <typename T>
+__device__ __forceinline__ void stream_out(T* p, const Vec<T>& v) {
+  using Bits = __attribute__((ext_vector_type(4))) unsigned;
+  __builtin_nontemporal_store(__builtin_bit_cast(Bits, v), reinterpret_cast<Bits*>(p));
+}
+
 // This thread's share of a list, every kThreads-th entry: the first kHeld in
 // registers, requested together, the others when they are looked at.
 template <int kHeld>
@@ -67,9 +76,9 @@ __global__ __launch_bounds__(kThreads, 8) void logits_kernel(fah_logits_adjust a
   // bit 31 whether it is in the history at all; `entry` its last bias entry plus
   // one. A window of one chunk has a slot a place. For several chunks at once the
   // slots are those of the named places in turn, `start` where each word's
-  // begin: the lists are looked through once (256 rows of 151936 in bf16: 47.6
-  // us, 51 chunk by chunk; without lists 37). Integer atomics: no order changes
-  // the result.
+  // begin: the lists are looked through once (256 rows of 151936 in bf16, stores
+  // through the caches: 47.6 us, 51 chunk by chunk). Integer atomics: no order
+  // changes the result.
   struct Table {
     unsigned seen[kChunk], entry[kChunk], named[kWords], start[kWords];
   };
@@ -240,7 +249,7 @@ __global__ __launch_bounds__(kThreads, 8) void logits_kernel(fah_logits_adjust a
         }
       }
       if (out_alike) {
-        *reinterpret_cast<Vec<T>*>(out + t) = g.x;
+        stream_out(out + t, g.x);
       } else {
 #pragma unroll
         for (int e = 0; e < V; ++e) out[t + e] = g.x.v[e];
@@ -285,8 +294,8 @@ struct ChoiceCut {
 
 // As many workgroups as the chip holds at once (8 a CU) have one chunk each;
 // with more, a workgroup takes up to four, so that looking the lists up once
-// serves them all (256 rows of 151936 in bf16: 63 us with one chunk, 48.7 with
-// three, 47.6 with four, 52 with eight, 57 with sixteen).
+// serves them all (256 rows of 151936 in bf16: 33.4 us with four chunks, 35.3
+// with three or five, 35 with eight).
 constexpr int kGroups = 2048;
 
 ChoiceCut choice_cut(const fah_logits_adjust& a) {
