@@ -442,6 +442,38 @@ def test_prefix_large(backend, types, count, prefix, longest, heads, kv_heads, s
     check_prefix(got[some], arrays[0][some], *arrays[1:3], arrays[3][some], arrays[4][some], lengths[some], types)
 
 
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(t))
+@pytest.mark.parametrize("count,heads,kv_heads,size", [(300, 4, 2, 128), (1100, 64, 2, 128), (300, 4, 4, 96)], ids=str)
+def test_prefix_capacities_past_the_caches(backend, types, count, heads, kv_heads, size):
+    """Own rows that count as more than the caches hold; the sequences' cache rows overlap, 16 apart."""
+    from funasrnet_amd import hip
+    rng = np.random.default_rng(count + size)
+    capacity, step, prefix = 4096, 16, 100
+    rows = capacity + step * count
+    q = store(rng.standard_normal((count, heads, size)) * 1.5, types[0])
+    pk, pv = (store(rng.standard_normal((prefix, kv_heads, size)), types[1]) for _ in range(2))
+    k, v = (store(rng.standard_normal((rows, kv_heads, size)), types[1]) for _ in range(2))
+    lengths = np.where(rng.random(count) < 0.02, capacity, rng.integers(0, 200, count)).astype(np.int32)
+    dq, dpk, dpv, dk, dv, dl = (to_device(x) for x in (q, pk, pv, k, v, lengths))
+    out = to_device(np.full_like(q, 55))
+    line = kv_heads * size
+    call = hip.PrefixAttention(
+        query=dq.ptr, prefix_key=dpk.ptr, prefix_value=dpv.ptr, key=dk.ptr, value=dv.ptr, output=out.ptr, lengths=dl.ptr,
+        query_sequence=heads * size, query_head=size, prefix_key_row=line, prefix_key_head=size, prefix_value_row=line,
+        prefix_value_head=size, key_sequence=step * line, key_row=line, key_head=size, value_sequence=step * line,
+        value_row=line, value_head=size, output_sequence=heads * size, output_head=size, sequences=count, prefix=prefix,
+        capacity=capacity, longest=capacity, heads=heads, kv_heads=kv_heads, head_size=size, query_type=CODES[types[0]],
+        cache_type=CODES[types[1]], scale=size**-0.5)
+    need = backend.attention_prefix_workspace(call)
+    ws = workspace_of(need)
+    call.workspace, call.workspace_bytes = ws.ptr, need
+    assert backend.attention_prefix_device(call) == hip.OK
+    backend.synchronize()
+    some = np.unique(np.concatenate([rng.integers(0, count, 12), np.flatnonzero(lengths == capacity)[:2], [0, count - 1]]))
+    own_k, own_v = (np.stack([a[step * i:step * i + capacity] for i in some]) for a in (k, v))
+    check_prefix(out.numpy()[some], q[some], pk, pv, own_k, own_v, lengths[some], types)
+
+
 @pytest.mark.parametrize("bad", [np.nan, np.inf])
 def test_prefix_rows_behind_the_length_may_hold_anything(backend, bad):
     types = ("f32", "f16")
