@@ -198,6 +198,8 @@ def _inputs(case: dict, seed: int) -> dict:
 
 
 def prepare(case: dict, seed: int) -> dict:
+    if own:
+        _backend()  # before the inputs: they are made on its stream
     v = _inputs(case, seed)
     # What the host knows of device-side lengths: bounds.
     state = {"case": case, **v}
@@ -215,10 +217,16 @@ _shared: dict = {}
 
 
 def _backend():
+    """The context. torch works on the context's stream from here on: inputs are
+    written before the calls that read them, outputs read after the calls that
+    write them, and tensors given back to the allocator while calls still use
+    them are not handed out to work ahead of those."""
     from funasrnet_amd import hip
 
     if "backend" not in _shared:
         _shared["backend"] = hip.HipBackend(0)
+        _shared["stream"] = torch.cuda.ExternalStream(_shared["backend"].stream, device=0)
+    torch.cuda.set_stream(_shared["stream"])
     return _shared["backend"], hip
 
 
