@@ -56,6 +56,12 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // down to 2^-22 of the largest one. The reference only moves when a row's
 // largest score has risen by more than kSlack.
 constexpr float kLift = 8.0f, kSlack = 6.0f;
+// A weight's exponent is formed as s c - (reference c) in one fma, which is off
+// by the rounding of the reference's product, the same for all of a row. From
+// this size on that rounding is a whole power of two and more, and weights would
+// overflow or vanish: there it is (s - reference) c, one instruction a score more
+// (not everywhere, for the vector units are half of what bounds long prompts).
+constexpr float kFar = 8388608.0f;
 
 __device__ __forceinline__ int clamp_int(int v, int low, int high) { return v < low ? low : v > high ? high : v; }
 
@@ -99,8 +105,8 @@ struct Task {
   __device__ __forceinline__ const Q* query(int r) const { return q + token(r) * q_token + head(r) * q_head; }
 };
 
-// Where it goes: the finished rows, or partial ones for a join: sums, each
-// row's reference (a power of two) and total.
+// Where it goes: the finished rows, or partial ones for a join: sums and total
+// of the weights 2^(c (s - mark)), and the mark, a score q k.
 template <typename Q>
 struct Sink {
   Q* out;                    // token 0, the K/V head's first query head; null: partial
@@ -211,7 +217,7 @@ struct Loader {
 
 // A row by one wave, channels 2 lane and 2 lane + 1, only keys that it sees
 // read: for rows whose tile held infinities or NaN where they are masked.
-// The lane's two sums, then the row's reference and total.
+// The lane's two sums, then the row's mark and total.
 template <typename Q, typename K>
 __device__ __noinline__ f32x4 slow_row(const Q* q, const K* k_rows, const K* v_rows, unsigned k_row, unsigned v_row, int begin,
                                        int lim, int size, float scale) {
@@ -228,10 +234,9 @@ __device__ __noinline__ f32x4 slow_row(const Q* q, const K* k_rows, const K* v_r
         v[i] = (float)w[2 * lane + i];
       }
     for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
-    s *= scale * kLog2e;
     const float next = s > top || s != s ? s : top;
-    const float base = next == -kInf ? 0.0f : next;
-    const float keep = __builtin_amdgcn_exp2f(top - base), p = __builtin_amdgcn_exp2f(s - base);
+    const float base = next == -kInf ? 0.0f : next, c = scale * kLog2e;
+    const float keep = __builtin_amdgcn_exp2f((top - base) * c), p = __builtin_amdgcn_exp2f((s - base) * c);
     total = total * keep + p;
     for (int i = 0; i < 2; ++i) sum[i] = sum[i] * keep + p * v[i];
     top = next;
@@ -312,7 +317,7 @@ struct Core {
     const int first_step = WR == 1 ? wave * kMine : 0;
     s16x8 part[kSplit ? 2 : 1][kMine];
     f32x4 raw[kSplit ? kMine : 1][2];
-    float c = scale * kLog2e;
+    float c = scale * kLog2e, unlift = 1.0f;  // (of a score of lifted queries)
     {
       const Q* q = t.query(valid ? my_row : 0);
 #pragma unroll
@@ -372,7 +377,8 @@ struct Core {
         part[0][s] = __builtin_bit_cast(s16x8, hi);
         part[kSplit ? 1 : 0][s] = __builtin_bit_cast(s16x8, lo);
       }
-      c = fmaxf(c * u2f((unsigned)(127 - up) << 23), 1.2e-38f);
+      unlift = u2f((unsigned)(127 - up) << 23);
+      c = fminf(fmaxf(c * unlift, 1.2e-38f), 3.4e38f);
     }
     s16x8 qf[kSplit ? 2 : 1][kSteps];
     if constexpr (WR == 1) {
@@ -397,8 +403,10 @@ struct Core {
     f32x16 acc[D / 32];
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) acc[i] = f32x16{};
-    float ref = -kInf, total = 0.0f;
-    bool masked = false;
+    float ref = -kInf, ref_c = -kInf, total = 0.0f;  // the reference, a score, and its product with c
+    bool masked = false, any_far = false;  // any_far: a row's reference is beyond kFar
+    // What a weight's exponent has over (s - reference) c.
+    auto lift = [&](float x, float x_c) { return fabsf(x_c) < kFar ? kLift + __builtin_fmaf(x, c, -x_c) : kLift; };
 
     // Fragment places within a tile. Keys: lane's row, chunk 2 s + half.
     // Values: lane 16 g + i of a half reads row i / 4 of four, 8 bytes of the
@@ -437,16 +445,30 @@ struct Core {
       for (int b = 0; b < NK / 32; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-      top = fmaxf(top, other_half(top)) * c;
-      const bool rise = top > ref + kSlack;
+      top = fmaxf(top, other_half(top));
+      const bool rise = (top - ref) * c > kSlack;
       if (__builtin_amdgcn_ballot_w64(rise) != 0) {
-        const float keep = rise ? __builtin_amdgcn_exp2f(ref - top) : 1.0f;
-        ref = rise ? top : ref;
+        const float next = rise ? top : ref, next_c = next * c;
+        const bool were_far = any_far;
+        // (Rows of infinite scores are zeros or NaN either way.)
+        any_far = __builtin_amdgcn_ballot_w64(fabsf(next_c) >= kFar && fabsf(next) < kInf) != 0;
+        float down = ref_c - next_c;
+        if (__builtin_expect(any_far || were_far, false)) down = (ref - next) * c + (lift(next, next_c) - lift(ref, ref_c));
+        const float keep = rise ? __builtin_amdgcn_exp2f(down) : 1.0f;
+        ref = next;
+        ref_c = next_c;
         total *= keep;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) acc[i] *= keep;
       }
-      const float base = ref == -kInf ? 0.0f : kLift - ref;
+      float base = ref == -kInf ? 0.0f : kLift - ref_c;
+      if (__builtin_expect(any_far, false)) {
+        base = lift(ref, ref_c);
+#pragma unroll
+        for (int b = 0; b < NK / 32; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[b][i] -= ref == -kInf ? 0.0f : ref;
+      }
 #pragma unroll
       for (int b = 0; b < NK / 32; ++b)
 #pragma unroll
@@ -524,12 +546,12 @@ struct Core {
       }
     }
     total += other_half(total);
+    const float unit = __builtin_amdgcn_exp2f(-lift(ref, ref_c));  // sums to those of the mark
 
     if constexpr (WK == 1) {
       // The rows are the wave's own: from registers to memory, a lane four
       // channels of eight, both halves together 16 or 32 bytes.
-      const float top = ref == -kInf ? ref : ref - kLift;
-      const float factor = !sink.out ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
+      const float factor = !sink.out ? unit : total == 0.0f ? 0.0f : 1.0f / total;
       bool bad = false;
       if (masked) {
         float most = 0.0f;
@@ -560,10 +582,10 @@ struct Core {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               *reinterpret_cast<f32x4*>(dst + 32 * i + 8 * j) =
-                  f32x4{acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]};
+                  f32x4{acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]} * factor;
           if (half == 0) {
-            sink.marks[2 * my_row] = top;
-            sink.marks[2 * my_row + 1] = total;
+            sink.marks[2 * my_row] = ref * unlift;
+            sink.marks[2 * my_row + 1] = total * factor;
           }
         }
       }
@@ -587,8 +609,8 @@ struct Core {
     // (to the finished row's scale where the row ends here) and leaves them in
     // LDS, [wave][32 rows][D] with the 16-byte chunks of a row swizzled.
     if (half == 0) {
-      marks[(wave * 32 + col) * 2] = ref - kLift;
-      marks[(wave * 32 + col) * 2 + 1] = total;
+      marks[(wave * 32 + col) * 2] = ref;
+      marks[(wave * 32 + col) * 2 + 1] = total * unit;
     }
     if (lane == 0) marks[64 * (kWaves + WR) + wave] = masked ? 1.0f : 0.0f;
     __syncthreads();
@@ -603,13 +625,13 @@ struct Core {
         m[w] = marks[((wr * WK + w) * 32 + col) * 2];
         top = fmaxf(top, m[w]);
       }
-      auto weight = [&](float x) { return x == -kInf ? 0.0f : x == top ? 1.0f : __builtin_amdgcn_exp2f(x - top); };
+      auto weight = [&](float x) { return x == -kInf ? 0.0f : x == top ? 1.0f : __builtin_amdgcn_exp2f((x - top) * c); };
 #pragma unroll
       for (int w = 0; w < WK; ++w) sum += weight(m[w]) * marks[((wr * WK + w) * 32 + col) * 2 + 1];
-      factor = weight(ref - kLift) * (sink.out ? sum == 0.0f ? 0.0f : 1.0f / sum : 1.0f);
+      factor = weight(ref) * unit * (sink.out ? sum == 0.0f ? 0.0f : 1.0f / sum : 1.0f);
     }
     if (half == 0 && wk == 0) {
-      marks[64 * kWaves + my_row * 2] = top;
+      marks[64 * kWaves + my_row * 2] = top * unlift;
       marks[64 * kWaves + my_row * 2 + 1] = sum;
     }
     if (valid) {
@@ -833,7 +855,8 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void packed_kernel(fah_packed_atte
 template <int D>
 struct Joined {
   static constexpr int kLanes = D / 4;
-  float top = -kInf, total = 0.0f;
+  float c;                           // exponents of two a score
+  float top = -kInf, total = 0.0f;   // the mark of what is joined so far
   f32x4 o = {};
   template <typename At, typename Marks>
   __device__ __forceinline__ void add(int count, At at, Marks marks) {
@@ -856,8 +879,8 @@ struct Joined {
       float next = fmaxf(top, m);
       for (int x = kLanes / 2; x >= 1; x >>= 1) next = fmaxf(next, __shfl_xor(next, x, kLanes));
       // A partial row that saw nothing counts as nothing, unless its total is NaN.
-      const float weight = m == -kInf ? 0.0f : m == next ? 1.0f : __builtin_amdgcn_exp2f(m - next);
-      const float keep = top == -kInf || top == next ? 1.0f : __builtin_amdgcn_exp2f(top - next);
+      const float weight = m == -kInf ? 0.0f : m == next ? 1.0f : __builtin_amdgcn_exp2f((m - next) * c);
+      const float keep = top == -kInf || top == next ? 1.0f : __builtin_amdgcn_exp2f((top - next) * c);
       float sum = w == w ? weight * w : w;
       for (int x = kLanes / 2; x >= 1; x >>= 1) sum += __shfl_xor(sum, x, kLanes);
       total = total * keep + sum;
@@ -895,7 +918,7 @@ __global__ __launch_bounds__(kThreads) void packed_join_kernel(fah_packed_attent
   const int shares = shares_of(visible_keys(p, group), cut);
   if (shares == 1) return;
   const float* sums = static_cast<const float*>(a.workspace) + ((size_t)slot * a.kv_heads + head) * cut.splits * BM * (D + 2);
-  Joined<D> j;
+  Joined<D> j{a.scale * kLog2e};
   j.add(shares, [&](int i) { return sums + (size_t)i * BM * (D + 2) + r * D + 4 * chunk; },
         [&](int i) { return sums + (size_t)i * BM * (D + 2) + BM * D + 2 * r; });
   const int row = p.row0 + r;
@@ -1002,7 +1025,7 @@ __global__ __launch_bounds__(kThreads) void prefix_join_kernel(fah_prefix_attent
   const float* own = static_cast<const float*>(a.workspace) + (size_t)a.kv_heads * shares * step +
                      ((size_t)s * a.kv_heads + head) * cut.own_shares * own_step;
   const int row = s * group + g;
-  Joined<D> j;
+  Joined<D> j{a.scale * kLog2e};
   j.add(shares + cut.own_shares,
         [&](int i) {
           return i < shares ? shared + i * step + (size_t)row * D + 4 * chunk

@@ -968,3 +968,82 @@ def test_decoder_choose(persistent, monkeypatch, oracle_lib):
         gpu.close()
         ref.close()
         backend.close()
+
+
+# ---- Scores and values far from 1 -------------------------------------------------------
+
+
+def whole_scores(rng, rows, keys, heads, kv_heads, size, types, shift):
+    """Queries and keys of few bits, so that every score is exact in 32 bits: `shift` powers of two times a whole number."""
+    limit = {"f32": 100, "f16": 13, "bf16": 60}[types[0]]
+    up = min(shift, limit)
+    q = store(rng.integers(-1, 2, (rows, heads, size)) * np.exp2(up), types[0])
+    k = store(rng.integers(-8, 9, (keys, kv_heads, size)) * np.exp2(shift - up), types[1])
+    return q, k
+
+
+def check_exact_scores(got, q, k, v, offset, types, scale, span):
+    """Scores without rounding errors: only those of the weights (of scores at most `span` below the largest), sums and output stay."""
+    heads, kv_heads, size = q.shape[1], k.shape[1], q.shape[2]
+    fq, fk, fv, fg = load(q, types[0]), load(k, types[1]), load(v, types[1]), load(got, types[0])
+    for h in range(heads):
+        g = h // (heads // kv_heads)
+        out, weight, _ = attend_all(fq[:, h], fk[:, g], fv[:, g], scale, offset)
+        off = np.abs(fg[:, h] - out)
+        limit = attention_bound(out, weight, span, len(k), size, types[0])
+        assert np.all(off <= limit), (h, float((off / limit).max()))
+
+
+@pytest.mark.parametrize("types,shifts", [(("f32", "f16"), (12, 20, 24, 28, 32, 40, 100)), (("f16", "f16"), (12, 20, 23)),
+                                          (("bf16", "bf16"), (12, 20, 24, 28, 32, 40, 100))], ids=lambda t: "-".join(map(str, t)))
+@pytest.mark.parametrize("rows,heads,kv_heads,extra", [(130, 2, 1, 0), (1100, 64, 64, 0), (40, 4, 2, 3000), (1, 4, 4, 500)])
+def test_packed_scores_of_any_size(backend, types, shifts, rows, heads, kv_heads, extra):
+    """From thousands to 2^100 and more: the keys with the largest score share the weight."""
+    for shift in shifts:
+        rng = np.random.default_rng(shift * 7 + rows)
+        print(f"scores {shift} {rows} {heads}/{kv_heads} {extra} {types}", flush=True)
+        q, k = whole_scores(rng, rows, rows + extra, heads, kv_heads, 128, types, shift)
+        v = store(rng.standard_normal(k.shape), types[1])
+        got = run_packed(backend, q, k, v, offsets([rows]), offsets([rows + extra]), types)
+        # (Other scores are at least 2^12 128^-0.5 below: weight 0.)
+        some = [0, 1, heads // 2, heads - 1] if heads > 4 else range(heads)
+        for h in some:
+            g = h // (heads // kv_heads)
+            check_exact_scores(got[:, h:h + 1], q[:, h:h + 1], k[:, g:g + 1], v[:, g:g + 1], extra, types, 128**-0.5, 1.0)
+
+
+def close_scores(rng, queries, keys, size, types, power, order):
+    """Scores 2^power + n units, n below 12, with the keys in the order of n or in any: a unit is the step of a 32-bit value there."""
+    unit = power - 23
+    n = rng.integers(0, 12, keys)
+    if order == "rising":
+        n.sort()
+    q, k = np.zeros((queries, 1, size)), np.zeros((keys, 1, size))
+    big = {"f32": 14, "f16": 14, "bf16": 40}[types[0]]
+    q[:, 0, 0], k[:, 0, 0] = np.exp2(min(big, power)), np.exp2(power - min(big, power))
+    q[:, 0, 1:3], k[:, 0, 1] = np.exp2(max(unit, 0)), n * np.exp2(min(unit, 0))
+    return store(q, types[0]), store(k, types[1])
+
+
+@pytest.mark.parametrize("types,powers", [(("f32", "f16"), (15, 22, 25, 27)), (("f16", "f16"), (15, 22, 25, 28)),
+                                          (("bf16", "bf16"), (15, 23, 28, 36, 60))], ids=lambda t: "-".join(map(str, t)))
+@pytest.mark.parametrize("order", ["rising", "any"])
+@pytest.mark.parametrize("unit", [0.02, 0.3, 2.0, 9.0])
+def test_scores_whose_differences_are_their_last_bits(backend, types, powers, order, unit):
+    """Scores of up to 2^27 and more after scaling, a few of their last bits apart: whole weights, and shares that agree."""
+    size = 64
+    for power in powers:
+        rng = np.random.default_rng(power)
+        scale = float(np.float32(unit * 2.0**(23 - power)))
+        for queries, keys in ((90, 90), (3, 1400)):
+            q, k = close_scores(rng, queries, keys, size, types, power, order)
+            v = store(rng.standard_normal(k.shape), types[1])
+            got = run_packed(backend, q, k, v, offsets([queries]), offsets([keys]), types, scale=scale)
+            check_exact_scores(got, q, k, v, keys - queries, types, scale, 12 * unit)
+        q, k = close_scores(rng, 5, 2100, size, types, power, order)
+        v = store(rng.standard_normal(k.shape), types[1])
+        lengths = np.array([100, 0, 37, 64, 1])
+        own_k, own_v = (np.stack([a[2000:]] * 5) for a in (k, v))
+        got = run_prefix(backend, q, k[:2000], v[:2000], own_k, own_v, lengths, types, scale=scale)
+        for s, n in enumerate(lengths):
+            check_exact_scores(got[s:s + 1], q[s:s + 1], k[:2000 + n], v[:2000 + n], 2000 + n, types, scale, 12 * unit)
