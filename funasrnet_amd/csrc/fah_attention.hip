@@ -51,11 +51,16 @@ using LdsFrag = s16x8 __attribute__((address_space(3))) *;
 constexpr int kThreads = 256;
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.44269504088896340736f;
-// Weights are held as 2^(score - reference + kLift): at most 2^(kLift + kSlack)
-// = 2^14, which fp16 holds, so that small weights keep fp16's full precision
-// down to 2^-22 of the largest one. The reference only moves when a row's
-// largest score has risen by more than kSlack.
-constexpr float kLift = 8.0f, kSlack = 6.0f;
+// Weights are held as 2^(score - reference + kLift). The reference only moves
+// when a row's largest score has risen by more than kSlack. For fp16 values they
+// are at most 2^(kLift + kSlack) = 2^14, which fp16 holds, so that small weights
+// keep fp16's full precision down to 2^-22 of the largest one. bf16 has the range
+// of fp32, and so have its values: there weights are at most 2^-18, so that the
+// sums of 2^17 of the largest values stay finite (values below 2^-102 lose bits
+// instead). Partial sums keep the lift, which the join divides out.
+constexpr float kSlack = 6.0f;
+template <typename K>
+constexpr float kLift = std::is_same_v<K, __bf16> ? -24.0f : 8.0f;
 // A weight's exponent is formed as s c - (reference c) in one fma, which is off
 // by the rounding of the reference's product, the same for all of a row. From
 // this size on that rounding is a whole power of two and more, and weights would
@@ -106,7 +111,7 @@ struct Task {
 };
 
 // Where it goes: the finished rows, or partial ones for a join: sums and total
-// of the weights 2^(c (s - mark)), and the mark, a score q k.
+// of the weights 2^(c (s - mark) + kLift), and the mark, a score q k.
 template <typename Q>
 struct Sink {
   Q* out;                    // token 0, the K/V head's first query head; null: partial
@@ -236,7 +241,7 @@ __device__ __noinline__ f32x4 slow_row(const Q* q, const K* k_rows, const K* v_r
     for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
     const float next = s > top || s != s ? s : top;
     const float base = next == -kInf ? 0.0f : next, c = scale * kLog2e;
-    const float keep = __builtin_amdgcn_exp2f((top - base) * c), p = __builtin_amdgcn_exp2f((s - base) * c);
+    const float keep = __builtin_amdgcn_exp2f((top - base) * c), p = __builtin_amdgcn_exp2f((s - base) * c + kLift<K>);
     total = total * keep + p;
     for (int i = 0; i < 2; ++i) sum[i] = sum[i] * keep + p * v[i];
     top = next;
@@ -405,8 +410,8 @@ struct Core {
     for (int i = 0; i < D / 32; ++i) acc[i] = f32x16{};
     float ref = -kInf, ref_c = -kInf, total = 0.0f;  // the reference, a score, and its product with c
     bool masked = false, any_far = false;  // any_far: a row's reference is beyond kFar
-    // What a weight's exponent has over (s - reference) c.
-    auto lift = [&](float x, float x_c) { return fabsf(x_c) < kFar ? kLift + __builtin_fmaf(x, c, -x_c) : kLift; };
+    // What a weight's exponent has over (s - reference) c + kLift.
+    auto over = [&](float x, float x_c) { return fabsf(x_c) < kFar ? __builtin_fmaf(x, c, -x_c) : 0.0f; };
 
     // Fragment places within a tile. Keys: lane's row, chunk 2 s + half.
     // Values: lane 16 g + i of a half reads row i / 4 of four, 8 bytes of the
@@ -453,7 +458,7 @@ struct Core {
         // (Rows of infinite scores are zeros or NaN either way.)
         any_far = __builtin_amdgcn_ballot_w64(fabsf(next_c) >= kFar && fabsf(next) < kInf) != 0;
         float down = ref_c - next_c;
-        if (__builtin_expect(any_far || were_far, false)) down = (ref - next) * c + (lift(next, next_c) - lift(ref, ref_c));
+        if (__builtin_expect(any_far || were_far, false)) down = (ref - next) * c + (over(next, next_c) - over(ref, ref_c));
         const float keep = rise ? __builtin_amdgcn_exp2f(down) : 1.0f;
         ref = next;
         ref_c = next_c;
@@ -461,9 +466,9 @@ struct Core {
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) acc[i] *= keep;
       }
-      float base = ref == -kInf ? 0.0f : kLift - ref_c;
+      float base = ref == -kInf ? 0.0f : kLift<K> - ref_c;
       if (__builtin_expect(any_far, false)) {
-        base = lift(ref, ref_c);
+        base = kLift<K> + over(ref, ref_c);
 #pragma unroll
         for (int b = 0; b < NK / 32; ++b)
 #pragma unroll
@@ -546,7 +551,7 @@ struct Core {
       }
     }
     total += other_half(total);
-    const float unit = __builtin_amdgcn_exp2f(-lift(ref, ref_c));  // sums to those of the mark
+    const float unit = __builtin_amdgcn_exp2f(-over(ref, ref_c));  // sums to those of the mark
 
     if constexpr (WK == 1) {
       // The rows are the wave's own: from registers to memory, a lane four

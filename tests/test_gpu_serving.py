@@ -1047,3 +1047,31 @@ def test_scores_whose_differences_are_their_last_bits(backend, types, powers, or
         got = run_prefix(backend, q, k[:2000], v[:2000], own_k, own_v, lengths, types, scale=scale)
         for s, n in enumerate(lengths):
             check_exact_scores(got[s:s + 1], q[s:s + 1], k[:2000 + n], v[:2000 + n], 2000 + n, types, scale, 12 * unit)
+
+
+@pytest.mark.parametrize("power", [126, 118, -112])
+@pytest.mark.parametrize("queries,keys,heads,kv_heads,size", [(130, 130, 4, 2, 128), (1100, 1100, 64, 64, 64), (9, 3000, 4, 2, 128)],
+                         ids=str)
+def test_bf16_values_of_any_size(backend, power, queries, keys, heads, kv_heads, size):
+    """Values near either end of the type's range: rows of every tile, and partial ones."""
+    types = ("bf16", "bf16")
+    q, k, v = packed_inputs(power + 200, [queries], [keys], heads, kv_heads, size, types)
+    v = store(np.clip(load(v, "bf16"), -3.5, 3.5) * np.float32(2.0**power), "bf16")
+    assert np.all(np.isfinite(load(v, "bf16")))
+    got = run_packed(backend, q, k, v, offsets([queries]), offsets([keys]), types)
+    fq, fk, fv, fg = load(q, "bf16"), load(k, "bf16"), load(v, "bf16") * 2.0**-power, load(got, "bf16") * 2.0**-power
+    for h in sorted({0, 1, heads - 1}):
+        g = h // (heads // kv_heads)
+        out, weight, dots = attend_all(fq[:, h], fk[:, g], fv[:, g], size**-0.5, keys - queries)
+        # Sums of small values end in the 32-bit numbers below the normal ones: a step of 2^-149 a key.
+        floor = 2.0 * keys * 2.0**(-149 + 24 - power) if power < 0 else 0.0
+        assert np.all(np.abs(fg[:, h] - out) <= attention_bound(out, weight, dots, keys, size, "bf16") + floor), h
+    lengths = [0, 1, 40, 70]
+    for prefix in (0, 2000):
+        q, pk, pv, k, v = prefix_inputs(power + 201, len(lengths), prefix, 70, heads, kv_heads, size, types)
+        pv, v = (store(np.clip(load(x, "bf16"), -3.5, 3.5) * np.float32(2.0**power), "bf16") for x in (pv, v))
+        got = run_prefix(backend, q, pk, pv, k, v, lengths, types)
+        assert np.all(np.isfinite(load(got, "bf16")))
+        if power > 0:
+            down = [store(load(x, "bf16") * np.float32(2.0**-power), "bf16") for x in (got, pv, v)]
+            check_prefix(down[0], q, pk, down[1], k, down[2], lengths, types)
