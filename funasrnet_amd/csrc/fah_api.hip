@@ -239,8 +239,10 @@ struct Ctx {
 // workgroup per CU, all co-resident, dealt to the XCDs in turn), so a
 // persistent section holds the lock from before its launches until its
 // stream has drained, after making its stream wait for the work already
-// enqueued on the other contexts' streams: no other context's kernel can
-// then run beside it.
+// enqueued on the other contexts' streams: no call of another context can
+// then put a kernel beside it. (Graphs that a caller replays and work that was
+// under way on a stream when its capture began are not waited for: kernels that
+// end leave the step its CUs, which it waits for.)
 struct DeviceGate {
   std::mutex m;
   std::vector<Ctx*> members;
@@ -292,6 +294,12 @@ struct PersistentSection {
   explicit PersistentSection(Ctx& ctx) : c(ctx), lock(device_gate(ctx.device).m) {
     for (Ctx* o : device_gate(c.device).members) {
       if (o == &c) continue;
+      // A stream under capture runs nothing, and a record would become a node of
+      // the caller's graph, the wait for it would draw this stream into the
+      // capture, and the step would be recorded there instead of run.
+      hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+      check(hipStreamIsCapturing(o->stream, &capture), "hipStreamIsCapturing");
+      if (capture != hipStreamCaptureStatusNone) continue;
       check(hipEventRecord(o->mark, o->stream), "hipEventRecord");
       check(hipStreamWaitEvent(c.stream, o->mark, 0), "hipStreamWaitEvent");
     }

@@ -22,8 +22,10 @@
  * enqueued under a per-device lock, and a persistent decode step or a
  * lock-step sessions step that runs the layers in one launch (both need
  * every CU of the device) first waits for the work already enqueued by the
- * other contexts and keeps the device to itself until it has finished, so
- * their kernels never run beside it.
+ * other contexts and keeps the device to itself until it has finished: calls
+ * of other contexts that enqueue wait until then, and no kernel of theirs runs
+ * beside it. It does not see graphs that a caller replays, nor a stream under
+ * capture.
  *
  * Lifetime: weights and decoders keep their context's state alive.
  * fah_context_destroy releases the handle (which must not be used again);
@@ -266,8 +268,10 @@ int fah_q8_block_dots_device(fah_context* context, const int8_t* q, const fah_we
  * The descriptors' pointers are device addresses on the context's device, and
  * their strides count elements. Work is ordered on the context stream (order
  * other streams with it through fah_context_stream and events); the calls
- * copy nothing, wait for nothing, allocate nothing and keep nothing, so they
- * may be captured into graphs. What they need beyond their outputs is the
+ * copy nothing, wait for no work of their stream, allocate nothing and keep
+ * nothing, so they may be captured into graphs, also while other contexts run
+ * decoder steps. (A call may have to wait until another context's persistent
+ * step has ended, as above.) What they need beyond their outputs is the
  * caller's `workspace`: at least the bytes that the *_workspace call of the
  * same descriptor gives (it needs no device and reads nothing through the
  * pointers), 16-byte aligned, its contents free before and after. Calls that

@@ -1075,3 +1075,51 @@ def test_bf16_values_of_any_size(backend, power, queries, keys, heads, kv_heads,
         if power > 0:
             down = [store(load(x, "bf16") * np.float32(2.0**-power), "bf16") for x in (got, pv, v)]
             check_prefix(down[0], q, pk, down[1], k, down[2], lengths, types)
+
+
+# ---- Captures beside another context's steps ------------------------------------------------
+
+
+@pytest.mark.parametrize("order", ["step first", "call first"])
+def test_capture_beside_another_contexts_steps(backend, order):
+    """A decoder of another context steps (persistent, lock-step) while the calls are captured: neither notices."""
+    import ctypes
+    from funasrnet_amd import device, hip, model
+    run, vp = device.runtime(), ctypes.c_void_p
+    weights = model.synthetic(model.small_config(layers=2, vocab=2048), seed=5)
+    x = np.random.default_rng(1).standard_normal((6, weights.config.width)).astype(np.float32)
+    other = hip.HipBackend(0)
+    decoder = hip.HipDecoder(other, weights, capacity=64)
+    s = Serving(backend, 61, count=4)
+    try:
+        def steps():
+            decoder.set_position(0)
+            decoder.decode(x, 6)
+            tokens = decoder.generate(3).tolist()
+            return tokens + hip.HipDecoder.generate_sessions([decoder], 3).reshape(-1).tolist() + [decoder.position]
+
+        expected = steps()
+        s.enqueue()
+        backend.synchronize()
+        results = s.results()
+        graph, made = vp(), vp()
+        assert run.hipStreamBeginCapture(vp(backend.stream), 2) == 0  # relaxed
+        if order == "call first":
+            s.enqueue()
+        print("steps beside a capture", flush=True)
+        assert steps() == expected
+        if order == "step first":
+            s.enqueue()
+        assert run.hipStreamEndCapture(vp(backend.stream), ctypes.byref(graph)) == 0
+        assert run.hipGraphInstantiate(ctypes.byref(made), graph, None, None, ctypes.c_size_t(0)) == 0
+        for _ in range(3):
+            s.clear()
+            assert run.hipGraphLaunch(made, vp(backend.stream)) == 0
+            backend.synchronize()
+            assert same(results, s.results())
+            assert steps() == expected
+        run.hipGraphExecDestroy(made)
+        run.hipGraphDestroy(graph)
+    finally:
+        decoder.close()
+        other.close()
