@@ -940,11 +940,12 @@ __global__ __launch_bounds__(kThreads) void packed_join_kernel(fah_packed_attent
 struct PrefixCut {
   int tiles, shares, own_tiles, own_shares;
   int64_t prefix_items, own_items;
+  int64_t prefix_rows, rows;  // partial rows of the prefix, and of all
 };
 
-// Partial rows: [K/V head][share][sequences * group][D + 2] of the prefix, then
-// [sequence][K/V head][own share][group][D + 2]; a row's sums, then its marks.
-// ONCE: own rows pass the caches by.
+// Partial rows: [K/V head][share][sequences * group] of the prefix, then
+// [sequence][K/V head][own share][group]. All rows' sums, [D] each and so on 16
+// bytes, then all rows' marks and totals. ONCE: own rows pass the caches by.
 template <typename Q, typename K, int D, int WR, int WK, int NK, bool ONCE>
 __global__ __launch_bounds__(kThreads, 2) void prefix_kernel(fah_prefix_attention a, PrefixCut cut) {
   using Shared = Core<Q, K, D, WR, WK, NK>;
@@ -977,9 +978,9 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_kernel(fah_prefix_attentio
     t.begin = share_at * share;
     t.end = t.begin + share < a.prefix ? t.begin + share : a.prefix;
     t.first_limit = t.end;
-    const size_t rows = ((size_t)head * cut.shares + share_at) * all;
-    sink.sums = partial + rows * (D + 2) + (size_t)row0 * D;
-    sink.marks = partial + rows * (D + 2) + (size_t)all * D + 2 * row0;
+    const size_t row = ((size_t)head * cut.shares + share_at) * all + row0;
+    sink.sums = partial + row * D;
+    sink.marks = partial + cut.rows * D + 2 * row;
     C::run(t, sink, a.head_size, a.scale, lds);
   } else {
     using C = Own;
@@ -1006,10 +1007,9 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_kernel(fah_prefix_attentio
       sink.o_token = a.output_sequence;
       sink.o_head = a.output_head;
     } else {
-      const size_t rows = (size_t)a.kv_heads * cut.shares * a.sequences * group * (cut.prefix_items ? 1 : 0) +
-                          (((size_t)s * a.kv_heads + head) * cut.own_shares + share_at) * group;
-      sink.sums = partial + rows * (D + 2) + (size_t)t.head0 * D;
-      sink.marks = partial + rows * (D + 2) + (size_t)group * D + 2 * t.head0;
+      const size_t row = cut.prefix_rows + (((size_t)s * a.kv_heads + head) * cut.own_shares + share_at) * group + t.head0;
+      sink.sums = partial + row * D;
+      sink.marks = partial + cut.rows * D + 2 * row;
     }
     C::run(t, sink, a.head_size, a.scale, lds);
   }
@@ -1025,21 +1025,13 @@ __global__ __launch_bounds__(kThreads) void prefix_join_kernel(fah_prefix_attent
   const int s = at / a.heads, q_head = at % a.heads, head = q_head / group, g = q_head % group;
   // The prefix's shares, then the own rows'.
   const int shares = cut.prefix_items ? cut.shares : 0;
-  const size_t step = (size_t)all * (D + 2), own_step = (size_t)group * (D + 2);
-  const float* shared = static_cast<const float*>(a.workspace) + (size_t)head * shares * step;
-  const float* own = static_cast<const float*>(a.workspace) + (size_t)a.kv_heads * shares * step +
-                     ((size_t)s * a.kv_heads + head) * cut.own_shares * own_step;
-  const int row = s * group + g;
+  const float* sums = static_cast<const float*>(a.workspace) + 4 * chunk;
+  const float* marks = static_cast<const float*>(a.workspace) + cut.rows * D;
+  const size_t first = (size_t)head * shares * all + s * group + g;
+  const size_t own = cut.prefix_rows + ((size_t)s * a.kv_heads + head) * cut.own_shares * group + g;
+  auto row = [&](int i) { return i < shares ? first + (size_t)i * all : own + (size_t)(i - shares) * group; };
   Joined<D> j{a.scale * kLog2e};
-  j.add(shares + cut.own_shares,
-        [&](int i) {
-          return i < shares ? shared + i * step + (size_t)row * D + 4 * chunk
-                            : own + (i - shares) * own_step + (size_t)g * D + 4 * chunk;
-        },
-        [&](int i) {
-          return i < shares ? shared + i * step + (size_t)all * D + 2 * row
-                            : own + (i - shares) * own_step + (size_t)group * D + 2 * g;
-        });
+  j.add(shares + cut.own_shares, [&](int i) { return sums + row(i) * D; }, [&](int i) { return marks + 2 * row(i); });
   if (4 * chunk < a.head_size) j.write(static_cast<Q*>(a.output) + s * a.output_sequence + q_head * a.output_head + 4 * chunk);
 }
 
@@ -1098,6 +1090,8 @@ PrefixCut prefix_cut(const fah_prefix_attention& a, int* waves_rows) {
   c.shares = (int)std::max<int64_t>({1, ceil_div(a.prefix, 4096), std::min<int64_t>(fill / (c.tiles * a.kv_heads), ceil_div(a.prefix, 256))});
   c.prefix_items = a.prefix ? (int64_t)c.tiles * a.kv_heads * c.shares : 0;
   c.own_items = own * c.own_shares;
+  c.prefix_rows = a.prefix ? (int64_t)c.shares * a.sequences * a.heads : 0;
+  c.rows = c.prefix_rows + (int64_t)c.own_shares * a.sequences * a.heads;
   return c;
 }
 
@@ -1164,8 +1158,7 @@ int64_t prefix_attention_workspace(const fah_prefix_attention& a) {
   int waves_rows;
   const PrefixCut c = prefix_cut(a, &waves_rows);
   if (!c.prefix_items && c.own_shares == 1) return 0;
-  const int64_t rows = ((c.prefix_items ? c.shares : 0) + c.own_shares) * (int64_t)a.sequences * a.heads;
-  return rows * (width_of(a.head_size) + 2) * 4;
+  return c.rows * (width_of(a.head_size) + 2) * 4;
 }
 
 hipError_t launch_packed_attention(const fah_packed_attention& a, hipStream_t s) {

@@ -500,6 +500,19 @@ def test_prefix_value_that_is_infinite(backend, prefix):
     assert np.all(np.isnan(got[2, 2:])) and np.all(np.isfinite(got[[0, 1, 3, 4], 2:]))
 
 
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(t))
+@pytest.mark.parametrize("count,heads,kv_heads", [(1, 1, 1), (3, 1, 1), (17, 6, 2), (5, 35, 7), (1, 3, 3)], ids=str)
+@pytest.mark.parametrize("size", [64, 104])
+def test_prefix_odd_partial_rows(backend, types, count, heads, kv_heads, size):
+    """Shares of both ranges whose rows are odd in number."""
+    rng = np.random.default_rng(count + heads)
+    lengths = rng.integers(0, 900, count)
+    lengths[0] = 900
+    arrays = prefix_inputs(count * heads, count, 1300, 900, heads, kv_heads, size, types)
+    got = run_prefix(backend, *arrays, lengths, types)
+    check_prefix(got, *arrays, lengths, types)
+
+
 def test_attention_is_deterministic(backend):
     types = ("f32", "f16")
     arrays = prefix_inputs(5, 20, 1800, 400, 8, 4, 128, types)
