@@ -220,33 +220,73 @@ struct Loader {
   }
 };
 
-// A row by one wave, channels 2 lane and 2 lane + 1, only keys that it sees
-// read: for rows whose tile held infinities or NaN where they are masked.
-// The lane's two sums, then the row's mark and total.
+// Whether a 16-bit value is infinite or NaN.
+template <typename K>
+__device__ __forceinline__ bool not_finite(K v) {
+  constexpr unsigned kExponent = std::is_same_v<K, __bf16> ? 0x7f80 : 0x7c00;
+  return (__builtin_bit_cast(unsigned short, v) & kExponent) == kExponent;
+}
+
+// A row's finished channels 2 lane and 2 lane + 1 by one wave, only keys that it
+// sees read: for those that infinite or NaN values reached from places which the
+// row's tiles masked, between `masked` and `last`. The last two values say which
+// channels these are; where there are none the row's own sums stand. A key a lane
+// for the scores, two channels a lane for the values; over once every channel
+// asked for is NaN. (24 prompts of 5014 rows, fp16, every value NaN: 1.3 ms, 12
+// key by key; one channel infinite everywhere 5.4; the first key alone 0.1.)
 template <typename Q, typename K>
 __device__ __noinline__ f32x4 slow_row(const Q* q, const K* k_rows, const K* v_rows, unsigned k_row, unsigned v_row, int begin,
-                                       int lim, int size, float scale) {
-  const int lane = threadIdx.x & 63;
-  float x[2] = {}, sum[2] = {}, top = -kInf, total = 0.0f;
-  for (int i = 0; i < 2; ++i)
-    if (2 * lane + i < size) x[i] = (float)q[2 * lane + i];
-  for (int key = begin; key < lim; ++key) {
-    const K *k = k_rows + (int64_t)key * k_row, *w = v_rows + (int64_t)key * v_row;
-    float s = 0.0f, v[2] = {};
-    for (int i = 0; i < 2; ++i)
-      if (2 * lane + i < size) {
-        s += x[i] * (float)k[2 * lane + i];
-        v[i] = (float)w[2 * lane + i];
-      }
-    for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
-    const float next = s > top || s != s ? s : top;
-    const float base = next == -kInf ? 0.0f : next, c = scale * kLog2e;
-    const float keep = __builtin_amdgcn_exp2f((top - base) * c), p = __builtin_amdgcn_exp2f((s - base) * c + kLift<K>);
-    total = total * keep + p;
-    for (int i = 0; i < 2; ++i) sum[i] = sum[i] * keep + p * v[i];
-    top = next;
+                                       int lim, int masked, int last, int size, float scale) {
+  const int lane = threadIdx.x & 63, d = 2 * lane;
+  const bool holds = d < size;  // (sizes are multiples of 8)
+  bool bad[2] = {};
+  for (int first = masked; first <= last; first += 16) {
+#pragma unroll 4
+    for (int key = first; key < first + 16; ++key)
+      if (holds && key <= last)
+        for (int i = 0; i < 2; ++i) bad[i] |= not_finite(v_rows[(int64_t)key * v_row + d + i]);
+    if (__builtin_amdgcn_ballot_w64(holds && !(bad[0] && bad[1])) == 0) break;
   }
-  return f32x4{sum[0], sum[1], top, total};
+  if (__builtin_amdgcn_ballot_w64(bad[0] || bad[1]) == 0) return f32x4{};
+  const float c = scale * kLog2e;
+  float sum[2] = {}, top = -kInf, total = 0.0f;
+  for (int first = begin; first < lim; first += 64) {
+    const int n = lim - first < 64 ? lim - first : 64;
+    float s = 0.0f;
+    const K* k = k_rows + (int64_t)(first + (lane < n ? lane : n - 1)) * k_row;
+    for (int e = 0; e < size; e += 8) {
+      alignas(16) K part[8];
+      *reinterpret_cast<uint4*>(part) = *reinterpret_cast<const uint4*>(k + e);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += (float)q[e + i] * (float)part[i];
+    }
+    if (lane >= n) s = -kInf;
+    float next = fmaxf(top, s);  // (NaN scores make the total NaN below)
+    for (int x = 32; x >= 1; x >>= 1) next = fmaxf(next, __shfl_xor(next, x, 64));
+    const float base = next == -kInf ? 0.0f : next, keep = __builtin_amdgcn_exp2f((top - base) * c);
+    const float p = lane < n ? __builtin_amdgcn_exp2f((s - base) * c + kLift<K>) : 0.0f;
+    float add = p;
+    for (int x = 32; x >= 1; x >>= 1) add += __shfl_xor(add, x, 64);
+    total = total * keep + add;
+    sum[0] *= keep;
+    sum[1] *= keep;
+    const K* v = v_rows + (int64_t)first * v_row + d;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const float w = __shfl(p, j, 64);
+      if (holds) {
+        sum[0] += w * (float)v[(int64_t)j * v_row];
+        sum[1] += w * (float)v[(int64_t)j * v_row + 1];
+      }
+    }
+    top = next;
+    bool open = false;
+    for (int i = 0; i < 2; ++i) open |= bad[i] && sum[i] == sum[i];
+    if (total != total || (total != 0.0f && __builtin_amdgcn_ballot_w64(open) == 0)) break;
+  }
+  if (total == 0.0f) sum[0] = sum[1] = 0.0f;
+  else sum[0] /= total, sum[1] /= total;
+  return f32x4{sum[0], sum[1], bad[0] ? 1.0f : 0.0f, bad[1] ? 1.0f : 0.0f};
 }
 
 // A 16-bit type's packed pair.
@@ -280,6 +320,13 @@ struct Core {
   static constexpr bool kSplit = std::is_same_v<Q, float>;
   static constexpr int kSteps = D / 16, kShared = WR == 1 ? kSteps * 1024 * (kSplit ? 2 : 1) : 0, kMarks = 8 * 32 * (kWaves + WR) + 4 * kWaves;
   static constexpr int kLds = kArea + (kShared > kMarks ? kShared : kMarks);
+
+  // slow_row for row r of the workgroup. Masked places: from the row's first
+  // unseen key on, and the last key, which is repeated behind it.
+  __device__ static f32x4 repaired(const Task<Q, K>& t, int r, int masked_last, int size, float scale) {
+    const int lim = t.limit(r), from = lim < t.end - 1 ? lim : t.end - 1;
+    return slow_row(t.query(r), t.k, t.v, t.k_row, t.v_row, t.begin, lim, from > t.begin ? from : t.begin, masked_last, size, scale);
+  }
 
   // lds: one or two buffers of a key tile and a value tile; at the end the
   // waves' sums. Behind them marks: [kWaves][32][2] of the waves, then [BM][2]
@@ -553,6 +600,9 @@ struct Core {
     total += other_half(total);
     const float unit = __builtin_amdgcn_exp2f(-over(ref, ref_c));  // sums to those of the mark
 
+    // The last key that a tile with masked places can have held.
+    const int tiles_end = t.begin + (end - t.begin + TR - 1) / TR * TR, masked_last = tiles_end <= last ? tiles_end - 1 : last;
+
     if constexpr (WK == 1) {
       // The rows are the wave's own: from registers to memory, a lane four
       // channels of eight, both halves together 16 or 32 bytes.
@@ -567,7 +617,7 @@ struct Core {
             if (D == size || 32 * i + 8 * (j >> 2) + 4 * half < size) most += fabsf(acc[i][j]);
         bad = valid && !(most + other_half(most) < kInf);
       }
-      if (valid && !bad) {
+      if (valid) {
         if (sink.out) {
           Q* dst = sink.out + t.token(my_row) * sink.o_token + t.head(my_row) * sink.o_head + 4 * half;
 #pragma unroll
@@ -594,18 +644,17 @@ struct Core {
           }
         }
       }
-      for (unsigned rows_bad = (unsigned)__builtin_amdgcn_ballot_w64(bad); rows_bad != 0; rows_bad &= rows_bad - 1) {
-        const int r = wr * 32 + __builtin_ctz(rows_bad);
-        const f32x4 v = slow_row(t.query(r), t.k, t.v, t.k_row, t.v_row, t.begin, t.limit(r), size, scale);
+      unsigned rows_bad = (unsigned)__builtin_amdgcn_ballot_w64(bad);
+      if (rows_bad != 0) __threadfence_block();  // the stores above come first
+      for (; rows_bad != 0; rows_bad &= rows_bad - 1) {
+        const int r = __builtin_ctz(rows_bad), row = wr * 32 + r;
+        const float whole = __shfl(total * factor, r, 64);
+        const f32x4 v = repaired(t, row, masked_last, size, scale);
         for (int i = 0; i < 2; ++i) {
           const int d = 2 * lane + i;
-          if (d >= size) continue;
-          if (sink.out) sink.out[t.token(r) * sink.o_token + t.head(r) * sink.o_head + d] = (Q)(v[3] == 0.0f ? 0.0f : v[i] / v[3]);
-          else sink.sums[(size_t)r * D + d] = v[i];
-        }
-        if (!sink.out && lane == 0) {
-          sink.marks[2 * r] = v[2];
-          sink.marks[2 * r + 1] = v[3];
+          if (v[2 + i] == 0.0f) continue;
+          if (sink.out) sink.out[t.token(row) * sink.o_token + t.head(row) * sink.o_head + d] = (Q)v[i];
+          else sink.sums[(size_t)row * D + d] = v[i] * whole;
         }
       }
       return;
@@ -668,13 +717,12 @@ struct Core {
           for (int g = 0; g < kAt; ++g) {
             if (!(bad >> (g * kLanes) & (kLanes == 64 ? ~0ull : (1ull << kLanes) - 1))) continue;
             const int row = r - lane / kLanes + g;
-            const f32x4 v = slow_row(t.query(row), t.k, t.v, t.k_row, t.v_row, t.begin, t.limit(row), size, scale);
+            const f32x4 v = repaired(t, row, masked_last, size, scale);
             // Lane l holds channels 2 l, 2 l + 1.
-            f32x4 w;
-            for (int i = 0; i < 4; ++i) w[i] = __shfl(i & 1 ? v[1] : v[0], 2 * chunk + (i >> 1), 64);
-            if (lane / kLanes == g) {
-              o = sink.out ? w * (v[3] == 0.0f ? 0.0f : 1.0f / v[3]) : w;
-              mark = f32x4{v[2], v[3]};
+            for (int i = 0; i < 4; ++i) {
+              const float w = __shfl(i & 1 ? v[1] : v[0], 2 * chunk + (i >> 1), 64);
+              const float bad_channel = __shfl(i & 1 ? v[3] : v[2], 2 * chunk + (i >> 1), 64);
+              if (lane / kLanes == g && bad_channel != 0.0f) o[i] = sink.out ? w : w * mark[1];
             }
           }
         }

@@ -1090,6 +1090,45 @@ def test_bf16_values_of_any_size(backend, power, queries, keys, heads, kv_heads,
             check_prefix(down[0], q, pk, down[1], k, down[2], lengths, types)
 
 
+# ---- Values that are not finite ------------------------------------------------------------
+
+
+@pytest.mark.parametrize("types", TYPES[1:], ids=lambda t: "-".join(t))
+@pytest.mark.parametrize("rows,extra,heads,kv_heads,size", [(40, 0, 2, 2, 128), (300, 0, 6, 2, 64), (1100, 0, 64, 64, 128), (400, 2500, 64, 64, 64),
+                                                            (60, 2000, 8, 4, 104), (5, 900, 4, 4, 128)], ids=str)
+def test_values_that_are_not_finite(backend, types, rows, extra, heads, kv_heads, size):
+    """Each channel by itself: NaN or infinite from the first key that holds one on, whatever its tile masks, and as ever in the others."""
+    keys = rows + extra
+    q, k, v = packed_inputs(rows + size, [rows], [keys], heads, kv_heads, size, types)
+    late = [keys - 1 - n for n in (0, min(rows - 1, 3), rows // 2, rows - 1)]  # keys that some rows see
+    spoilt = load(v, types[1]).astype(np.float32)
+    spoilt[0, :, 2], spoilt[:, :, 5] = np.nan, np.inf                # from the first key on; everywhere
+    spoilt[extra // 2, :, 7] = -np.inf
+    spoilt[late[1], :, 11], spoilt[late[2], :, 13], spoilt[late[3], :, 17] = np.nan, np.inf, -np.inf
+    spoilt[late[0]] = np.nan                                         # the last key: one row alone
+    clean = np.where(np.isfinite(spoilt), spoilt, 0.0)
+    got = load(run_packed(backend, q, k, store(spoilt, types[1]), offsets([rows]), offsets([keys]), types), types[0])
+    fq, fk = load(q, types[0]), load(k, types[1])
+    seen = np.arange(keys)[None, :] <= np.arange(rows)[:, None] + extra
+    for h in sorted({0, 1, heads // 2, heads - 1}):
+        g = h // (heads // kv_heads)
+        out, weight, dots = attend_all(fq[:, h], fk[:, g], clean[:, g], size**-0.5, extra)
+        limit = attention_bound(out, weight, dots, keys, size, types[0])
+        for kind, test in (("nan", np.isnan), ("inf", np.isposinf), ("-inf", np.isneginf)):
+            spoilt_by = (seen.astype(np.float32) @ test(spoilt[:, g]).astype(np.float32)) > 0  # [rows, size]
+            if kind == "nan":
+                nan = spoilt_by
+            elif kind == "inf":
+                up = spoilt_by
+            else:
+                down = spoilt_by
+        nan |= up & down
+        assert np.array_equal(np.isnan(got[:, h]), nan), h
+        assert np.array_equal(np.isposinf(got[:, h]), up & ~nan) and np.array_equal(np.isneginf(got[:, h]), down & ~nan), h
+        finite = ~(nan | up | down)
+        assert np.all(np.abs(got[:, h] - out)[finite] <= limit[finite]), h
+
+
 # ---- Captures beside another context's steps ------------------------------------------------
 
 
