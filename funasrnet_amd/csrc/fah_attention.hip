@@ -607,6 +607,10 @@ struct Core {
       // The rows are the wave's own: from registers to memory, a lane four
       // channels of eight, both halves together 16 or 32 bytes.
       const float factor = !sink.out ? unit : total == 0.0f ? 0.0f : 1.0f / total;
+      // A row that saw nothing is zeros, also where its values are not finite.
+      if (total == 0.0f)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) acc[i] = f32x16{};
       bool bad = false;
       if (masked) {
         float most = 0.0f;
@@ -688,6 +692,10 @@ struct Core {
       marks[64 * kWaves + my_row * 2] = top * unlift;
       marks[64 * kWaves + my_row * 2 + 1] = sum;
     }
+    // A share that saw nothing is zeros, also where its values are not finite.
+    if (factor == 0.0f)
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) acc[i] = f32x16{};
     if (valid) {
       float* sums = reinterpret_cast<float*>(lds) + (wave * 32 + col) * D;
 #pragma unroll

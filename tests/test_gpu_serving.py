@@ -1129,6 +1129,25 @@ def test_values_that_are_not_finite(backend, types, rows, extra, heads, kv_heads
         assert np.all(np.abs(got[:, h] - out)[finite] <= limit[finite]), h
 
 
+@pytest.mark.parametrize("types", TYPES[1:], ids=lambda t: "-".join(t))
+@pytest.mark.parametrize("rows,extra,heads,kv_heads", [(150, 0, 2, 2), (1100, 0, 64, 64), (70, 3000, 4, 2)], ids=str)
+def test_rows_of_minus_infinity_scores_over_any_values(backend, types, rows, extra, heads, kv_heads):
+    """Zeros, whatever the values are."""
+    q, k, v = packed_inputs(rows, [rows], [rows + extra], heads, kv_heads, 64, types)
+    q[:] = store(np.abs(load(q, types[0])) + 0.1, types[0])
+    k[:] = store(np.full(k.shape, -np.inf), types[1])
+    v[::3] = store(np.full(v[::3].shape, np.nan), types[1])
+    v[1::3] = store(np.full(v[1::3].shape, np.inf), types[1])
+    got = load(run_packed(backend, q, k, v, offsets([rows]), offsets([rows + extra]), types), types[0])
+    assert np.all(got == 0)
+    for prefix in (0, 1500):
+        q, pk, pv, k, v = prefix_inputs(9, 3, prefix, 90, heads, kv_heads, 64, types)
+        q = store(np.abs(load(q, types[0])) + 0.1, types[0])
+        pk, k = (store(np.full(x.shape, -np.inf), types[1]) for x in (pk, k))
+        pv, v = (store(np.full(x.shape, np.nan), types[1]) for x in (pv, v))
+        assert np.all(load(run_prefix(backend, q, pk, pv, k, v, [90, 0, 33], types), types[0]) == 0)
+
+
 # ---- Captures beside another context's steps ------------------------------------------------
 
 
