@@ -24,6 +24,8 @@
 // inputs has not, and adds to the error what rounding the output does: measured
 // 2.3e-3 of the result in bf16 against 1.7e-3. fp32 queries, and the weights of
 // their rows, are split into two fp16 parts and take two products each: 3e-7.
+// (Second parts may be 0 or of the other sign, which makes infinite keys and
+// values NaN: the rows are formed again in slow_row.)
 //
 // What bounds it: long prompts the matrix instructions and the card's power
 // (8192 rows of 32/8 heads in bf16: 525 us, 1.05 PFLOP/s, matrix units 52% busy
@@ -227,27 +229,33 @@ __device__ __forceinline__ bool not_finite(K v) {
   return (__builtin_bit_cast(unsigned short, v) & kExponent) == kExponent;
 }
 
-// A row's finished channels 2 lane and 2 lane + 1 by one wave, only keys that it
-// sees read: for those that infinite or NaN values reached from places which the
-// row's tiles masked, between `masked` and `last`. The last two values say which
-// channels these are; where there are none the row's own sums stand. A key a lane
+// A row that slow_row formed: the lane's channels 2 lane and 2 lane + 1, finished,
+// which of them stand in for the row's own, and its mark and total (see Sink).
+struct SlowRow {
+  float value[2], mark, total;
+  bool bad[2];
+};
+
+// A row by one wave, only keys that it sees read: all channels, or those that
+// infinite or NaN values between `masked` and `last` can have reached, which the
+// row's tiles masked or took in two parts. A key a lane
 // for the scores, two channels a lane for the values; over once every channel
 // asked for is NaN. (24 prompts of 5014 rows, fp16, every value NaN: 1.3 ms, 12
 // key by key; one channel infinite everywhere 5.4; the first key alone 0.1.)
 template <typename Q, typename K>
-__device__ __noinline__ f32x4 slow_row(const Q* q, const K* k_rows, const K* v_rows, unsigned k_row, unsigned v_row, int begin,
-                                       int lim, int masked, int last, int size, float scale) {
+__device__ __noinline__ SlowRow slow_row(const Q* q, const K* k_rows, const K* v_rows, unsigned k_row, unsigned v_row, int begin,
+                                         int lim, bool all, int masked, int last, int size, float scale) {
   const int lane = threadIdx.x & 63, d = 2 * lane;
   const bool holds = d < size;  // (sizes are multiples of 8)
-  bool bad[2] = {};
-  for (int first = masked; first <= last; first += 16) {
+  bool bad[2] = {all && holds, all && holds};
+  for (int first = masked; !all && first <= last; first += 16) {
 #pragma unroll 4
     for (int key = first; key < first + 16; ++key)
       if (holds && key <= last)
         for (int i = 0; i < 2; ++i) bad[i] |= not_finite(v_rows[(int64_t)key * v_row + d + i]);
     if (__builtin_amdgcn_ballot_w64(holds && !(bad[0] && bad[1])) == 0) break;
   }
-  if (__builtin_amdgcn_ballot_w64(bad[0] || bad[1]) == 0) return f32x4{};
+  if (__builtin_amdgcn_ballot_w64(bad[0] || bad[1]) == 0) return {};
   const float c = scale * kLog2e;
   float sum[2] = {}, top = -kInf, total = 0.0f;
   for (int first = begin; first < lim; first += 64) {
@@ -286,7 +294,7 @@ __device__ __noinline__ f32x4 slow_row(const Q* q, const K* k_rows, const K* v_r
   }
   if (total == 0.0f) sum[0] = sum[1] = 0.0f;
   else sum[0] /= total, sum[1] /= total;
-  return f32x4{sum[0], sum[1], bad[0] ? 1.0f : 0.0f, bad[1] ? 1.0f : 0.0f};
+  return {{sum[0], sum[1]}, top, total, {bad[0], bad[1]}};
 }
 
 // A 16-bit type's packed pair.
@@ -321,11 +329,12 @@ struct Core {
   static constexpr int kSteps = D / 16, kShared = WR == 1 ? kSteps * 1024 * (kSplit ? 2 : 1) : 0, kMarks = 8 * 32 * (kWaves + WR) + 4 * kWaves;
   static constexpr int kLds = kArea + (kShared > kMarks ? kShared : kMarks);
 
-  // slow_row for row r of the workgroup. Masked places: from the row's first
-  // unseen key on, and the last key, which is repeated behind it.
-  __device__ static f32x4 repaired(const Task<Q, K>& t, int r, int masked_last, int size, float scale) {
-    const int lim = t.limit(r), from = lim < t.end - 1 ? lim : t.end - 1;
-    return slow_row(t.query(r), t.k, t.v, t.k_row, t.v_row, t.begin, lim, from > t.begin ? from : t.begin, masked_last, size, scale);
+  // slow_row for row r of the workgroup with this total. Masked places: from the
+  // row's first unseen key on, and the last key, which is repeated behind it.
+  __device__ static SlowRow repaired(const Task<Q, K>& t, int r, float total, int masked_last, int size, float scale) {
+    const int lim = t.limit(r), from = kSplit ? t.begin : lim < t.end - 1 ? lim : t.end - 1;
+    return slow_row(t.query(r), t.k, t.v, t.k_row, t.v_row, t.begin, lim, kSplit && total != total,
+                    from > t.begin ? from : t.begin, masked_last, size, scale);
   }
 
   // lds: one or two buffers of a key tile and a value tile; at the end the
@@ -612,14 +621,14 @@ struct Core {
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) acc[i] = f32x16{};
       bool bad = false;
-      if (masked) {
+      if (masked || kSplit) {
         float most = 0.0f;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i)
 #pragma unroll
           for (int j = 0; j < 16; ++j)
             if (D == size || 32 * i + 8 * (j >> 2) + 4 * half < size) most += fabsf(acc[i][j]);
-        bad = valid && !(most + other_half(most) < kInf);
+        bad = valid && !(most + other_half(most) < kInf) && (kSplit || total == total);
       }
       if (valid) {
         if (sink.out) {
@@ -653,12 +662,17 @@ struct Core {
       for (; rows_bad != 0; rows_bad &= rows_bad - 1) {
         const int r = __builtin_ctz(rows_bad), row = wr * 32 + r;
         const float whole = __shfl(total * factor, r, 64);
-        const f32x4 v = repaired(t, row, masked_last, size, scale);
+        const SlowRow v = repaired(t, row, whole, masked_last, size, scale);
+        const bool all = whole != whole;
         for (int i = 0; i < 2; ++i) {
           const int d = 2 * lane + i;
-          if (v[2 + i] == 0.0f) continue;
-          if (sink.out) sink.out[t.token(row) * sink.o_token + t.head(row) * sink.o_head + d] = (Q)v[i];
-          else sink.sums[(size_t)row * D + d] = v[i] * whole;
+          if (!v.bad[i]) continue;
+          if (sink.out) sink.out[t.token(row) * sink.o_token + t.head(row) * sink.o_head + d] = (Q)v.value[i];
+          else sink.sums[(size_t)row * D + d] = v.value[i] * (all ? v.total : whole);
+        }
+        if (!sink.out && all && lane == 0) {
+          sink.marks[2 * row] = v.mark;
+          sink.marks[2 * row + 1] = v.total;
         }
       }
       return;
@@ -718,20 +732,25 @@ struct Core {
       const bool stored = r < t.rows && 4 * chunk < size;
       f32x4 mark = {};
       if (!sink.out) mark = f32x4{marks[64 * kWaves + 2 * r], marks[64 * kWaves + 2 * r + 1]};
-      if (any_masked) {
+      if (any_masked || kSplit) {
         const unsigned long long bad =
-            __builtin_amdgcn_ballot_w64(stored && !(fabsf(o[0]) + fabsf(o[1]) + fabsf(o[2]) + fabsf(o[3]) < kInf));
+            __builtin_amdgcn_ballot_w64(stored && (!(fabsf(o[0]) + fabsf(o[1]) + fabsf(o[2]) + fabsf(o[3]) < kInf) ||
+                                                   (kSplit && mark[1] != mark[1])));
         if (bad != 0) {
           for (int g = 0; g < kAt; ++g) {
             if (!(bad >> (g * kLanes) & (kLanes == 64 ? ~0ull : (1ull << kLanes) - 1))) continue;
             const int row = r - lane / kLanes + g;
-            const f32x4 v = repaired(t, row, masked_last, size, scale);
+            const float total = marks[64 * kWaves + 2 * row + 1];
+            if (!kSplit && total != total) continue;  // NaN as it should be
+            const SlowRow v = repaired(t, row, total, masked_last, size, scale);
+            const bool all = total != total;
             // Lane l holds channels 2 l, 2 l + 1.
             for (int i = 0; i < 4; ++i) {
-              const float w = __shfl(i & 1 ? v[1] : v[0], 2 * chunk + (i >> 1), 64);
-              const float bad_channel = __shfl(i & 1 ? v[3] : v[2], 2 * chunk + (i >> 1), 64);
-              if (lane / kLanes == g && bad_channel != 0.0f) o[i] = sink.out ? w : w * mark[1];
+              const float w = __shfl(v.value[i & 1], 2 * chunk + (i >> 1), 64);
+              const int stands = __shfl((int)v.bad[i & 1], 2 * chunk + (i >> 1), 64);
+              if (lane / kLanes == g && stands) o[i] = sink.out ? w : w * (all ? v.total : total);
             }
+            if (lane / kLanes == g && all) mark = f32x4{v.mark, v.total};
           }
         }
       }

@@ -1093,7 +1093,7 @@ def test_bf16_values_of_any_size(backend, power, queries, keys, heads, kv_heads,
 # ---- Values that are not finite ------------------------------------------------------------
 
 
-@pytest.mark.parametrize("types", TYPES[1:], ids=lambda t: "-".join(t))
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(t))
 @pytest.mark.parametrize("rows,extra,heads,kv_heads,size", [(40, 0, 2, 2, 128), (300, 0, 6, 2, 64), (1100, 0, 64, 64, 128), (400, 2500, 64, 64, 64),
                                                             (60, 2000, 8, 4, 104), (5, 900, 4, 4, 128)], ids=str)
 def test_values_that_are_not_finite(backend, types, rows, extra, heads, kv_heads, size):
@@ -1129,7 +1129,7 @@ def test_values_that_are_not_finite(backend, types, rows, extra, heads, kv_heads
         assert np.all(np.abs(got[:, h] - out)[finite] <= limit[finite]), h
 
 
-@pytest.mark.parametrize("types", TYPES[1:], ids=lambda t: "-".join(t))
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(t))
 @pytest.mark.parametrize("rows,extra,heads,kv_heads", [(150, 0, 2, 2), (1100, 0, 64, 64), (70, 3000, 4, 2)], ids=str)
 def test_rows_of_minus_infinity_scores_over_any_values(backend, types, rows, extra, heads, kv_heads):
     """Zeros, whatever the values are."""
@@ -1146,6 +1146,38 @@ def test_rows_of_minus_infinity_scores_over_any_values(backend, types, rows, ext
         pk, k = (store(np.full(x.shape, -np.inf), types[1]) for x in (pk, k))
         pv, v = (store(np.full(x.shape, np.nan), types[1]) for x in (pv, v))
         assert np.all(load(run_prefix(backend, q, pk, pv, k, v, [90, 0, 33], types), types[0]) == 0)
+
+
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(t))
+@pytest.mark.parametrize("rows,extra,heads,kv_heads,size", [(70, 0, 2, 2, 64), (1100, 0, 64, 64, 128), (400, 2500, 64, 64, 64), (60, 2000, 8, 4, 104),
+                                                            (3, 900, 4, 4, 128)], ids=str)
+def test_infinite_keys(backend, types, rows, extra, heads, kv_heads, size):
+    """Scores of -infinity weigh nothing, whatever their values are short of NaN and infinity; those of infinity make the row NaN."""
+    keys = rows + extra
+    q, k, v = packed_inputs(rows + 3, [rows], [keys], heads, kv_heads, size, types)
+    # Channel 5 of queries: above 0, but for every seventh row.
+    side = np.where(np.arange(rows) % 7 == 3, -1.0, 1.0)
+    q[:, :, 5] = store(side[:, None] * (np.abs(load(q[:, :, 5], types[0])) + 0.125), types[0])
+    k[::5, :, 5] = store(np.full(k[::5, :, 5].shape, -np.inf), types[1])
+    got = load(run_packed(backend, q, k, v, offsets([rows]), offsets([keys]), types), types[0])
+    fq, fk, fv = load(q, types[0]), load(k, types[1]), load(v, types[1])
+    at, others = np.arange(keys) % 5 != 0, side > 0
+    seen = np.arange(keys)[None, :] <= np.arange(rows)[:, None] + extra
+    for h in sorted({0, heads // 2, heads - 1}):
+        g = h // (heads // kv_heads)
+        assert np.all(np.isnan(got[~others, h])), h
+        for r in np.flatnonzero(others)[:: max(1, rows // 40)]:
+            out, weight, dots = attend(fq[r:r + 1, h], fk[at, g], fv[at, g], size**-0.5, seen[r:r + 1, at])
+            assert np.all(np.abs(got[r, h] - out[0]) <= attention_bound(out, weight, dots, keys, size, types[0])[0]), (h, r)
+    for prefix in (0, 1200):
+        lengths = [90, 1, 33]
+        q, pk, pv, k, v = prefix_inputs(10, 3, prefix, 90, heads, kv_heads, size, types)
+        q[:, :, 5] = store(np.abs(load(q[:, :, 5], types[0])) + 0.125, types[0])
+        drop = [np.arange(n) % 3 == 1 for n in (prefix, 90)]
+        pk[drop[0], :, 5], k[:, drop[1], :, 5] = (store(np.float32(-np.inf), types[1]) for _ in range(2))
+        got = run_prefix(backend, q, pk, pv, k, v, lengths, types)
+        kept = [int(np.sum(~drop[1][:n])) for n in lengths]
+        check_prefix(got, q, pk[~drop[0]], pv[~drop[0]], k[:, ~drop[1]], v[:, ~drop[1]], kept, types)
 
 
 # ---- Captures beside another context's steps ------------------------------------------------
