@@ -2148,8 +2148,9 @@ void require_workspace(const void* p, int64_t have, int64_t need) {
 // Most elements between two key or value rows: the kernels' offsets within 32
 // rows are byte offsets below 2^31.
 constexpr int64_t kRowStride = 1 << 25;
-// Most keys: a tile past the last one still counts in 32 bits.
-constexpr int kMostKeys = INT32_MAX - 4096;
+// Most keys: the ends of shares still count in 32 bits. A share is whole tiles of
+// at most 128 keys, so that the last of up to 2048 can end 2048 tiles past the keys.
+constexpr int kMostKeys = INT32_MAX - (1 << 19);
 
 // False: declined.
 bool check_packed(const fah_packed_attention& a) {

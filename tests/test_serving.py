@@ -93,3 +93,16 @@ def test_invalid_sizes_are_errors(kind, changes):
 def test_unsupported_forms_are_declined(kind, changes):
     rc, n = workspace(kind, **changes)
     assert rc == hip.DECLINED and n == -7
+
+
+@pytest.mark.parametrize("kind,size", [("packed", "key_rows"), ("prefix", "prefix"), ("prefix", "capacity")])
+def test_keys_whose_shares_end_past_32_bits(kind, size):
+    """256 shares of 2^31 - 4097 keys in tiles of 128 are 65536 tiles each: the last one's end, 2^31, is no 32-bit number."""
+    keys = 2**31 - 4097
+    tiles = -(-keys // 128)
+    assert -(-tiles // 256) * 128 * 256 == 2**31
+    rc, _ = workspace(kind, **{size: keys, "longest_key" if kind == "packed" else "longest": keys})
+    assert rc == hip.ERROR_ARGUMENT and b"keys" in hip.load().fah_last_error()
+    keys = 2**31 - 2**19 - 1
+    rc, _ = workspace(kind, **{size: keys, "longest_key" if kind == "packed" else "longest": keys})
+    assert rc == hip.OK
