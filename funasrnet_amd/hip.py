@@ -607,18 +607,22 @@ class HipDecoder:
         v = np.ascontiguousarray(list((biases or {}).values()), dtype=np.float32)
         words = None
         if mask is not None:
+            mask = np.asarray(mask)
             if mask.shape != (self.config.vocab,):
                 raise ValueError("the mask needs a truth value for each token")
             bits = np.zeros((self.config.vocab + 31) // 32 * 32, dtype=bool)
             bits[:self.config.vocab] = mask
             words = np.packbits(bits, bitorder="little").view(np.uint32)
-        if logits is not None and (logits.dtype != np.float32 or logits.size != self.config.vocab):
-            raise ValueError("logits must be float32 of the vocabulary's size")
+        if logits is not None and (logits.dtype != np.float32 or logits.size != self.config.vocab or not logits.flags.writeable):
+            raise ValueError("logits must be float32 of the vocabulary's size, and writeable")
+        out = None if logits is None else _Output(logits)
         token = ctypes.c_int32()
         _check(load().fah_decoder_choose(self.handle, _p(h, ctypes.c_int32), h.size, prompt, repetition, presence, frequency,
                                          _p(t, ctypes.c_int32), _p(v, ctypes.c_float), t.size,
                                          None if words is None else _p(words, ctypes.c_uint32),
-                                         None if logits is None else _p(logits, ctypes.c_float), ctypes.byref(token)))
+                                         None if out is None else out.pointer, ctypes.byref(token)))
+        if out is not None:
+            out.accept()
         return token.value
 
     def generate(self, steps: int) -> np.ndarray:

@@ -1,7 +1,9 @@
 """Refusals and sizes of the serving operators that need no device: the
 *_workspace calls check a descriptor as the device calls do."""
 import ctypes
+from types import SimpleNamespace
 
+import numpy as np
 import pytest
 
 from funasrnet_amd import hip
@@ -106,3 +108,36 @@ def test_keys_whose_shares_end_past_32_bits(kind, size):
     keys = 2**31 - 2**19 - 1
     rc, _ = workspace(kind, **{size: keys, "longest_key" if kind == "packed" else "longest": keys})
     assert rc == hip.OK
+
+
+def test_choose_arguments(monkeypatch):
+    """HipDecoder.choose: masks that are lists, logits that are not contiguous, and refusals ahead of the library's call."""
+    seen = {}
+
+    class Library:
+        @staticmethod
+        def fah_decoder_choose(handle, history, count, prompt, repetition, presence, frequency, tokens, values, biases, mask, out, token):
+            seen["mask"] = None if mask is None else [mask[0], mask[1]]
+            for i in range(40 if out is not None else 0):
+                out[i] = i + 0.5
+            token._obj.value = 7
+            return hip.OK
+
+    monkeypatch.setattr(hip, "load", lambda: Library)
+    decoder = object.__new__(hip.HipDecoder)
+    decoder.handle, decoder.config = 1, SimpleNamespace(vocab=40)
+    allowed = [i % 3 == 0 for i in range(40)]
+    assert decoder.choose([1, 2], mask=allowed) == 7
+    assert seen["mask"] == [sum(1 << i for i in range(0, 32, 3)), sum(1 << (i - 32) for i in range(33, 40, 3))]
+    wide = np.zeros((40, 2), np.float32)
+    assert decoder.choose(logits=wide[:, 1]) == 7
+    assert np.array_equal(wide[:, 1], np.arange(40) + 0.5) and np.all(wide[:, 0] == 0)
+    fixed = np.zeros(40, np.float32)
+    fixed.flags.writeable = False
+    seen.clear()
+    for bad in (dict(logits=fixed), dict(logits=np.zeros(40)), dict(logits=np.zeros(39, np.float32)), dict(mask=allowed[:39]),
+                dict(mask=np.ones((1, 40), bool))):
+        with pytest.raises(ValueError):
+            decoder.choose(**bad)
+    assert not seen and np.all(fixed == 0)
+    decoder.handle = None  # nothing to destroy
