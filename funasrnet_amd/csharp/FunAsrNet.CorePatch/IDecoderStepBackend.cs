@@ -26,4 +26,25 @@ public interface IDecoderStep : IDisposable
     /// <summary>The greedy token of the last decode's logits, then that token
     /// embedded and decoded (Greedy -> Embed -> Decode(1) on the device).</summary>
     int NextToken();
+    /// <summary>The greedy token of the last logits under <paramref name="rules"/>, which
+    /// the next NextToken returns and goes on from; -1 when nothing is left to choose.
+    /// The adjusted logits into <paramref name="logits"/> when it is not null.</summary>
+    int Choose(TokenRules rules, float[]? logits);
+}
+
+/// <summary>What <see cref="IDecoderStep.Choose"/> applies to the logits, in this order:
+/// penalties for the tokens of the history (its first PromptCount are the prompt),
+/// biases, and a grammar's mask (bit t % 32 of word t / 32 allows token t).</summary>
+public ref struct TokenRules
+{
+    public ReadOnlySpan<int> History;
+    public int PromptCount;
+    /// <summary>0 is taken as 1: no penalty.</summary>
+    public float Repetition;
+    public float Presence, Frequency;
+    public ReadOnlySpan<int> BiasTokens;
+    /// <summary>One for each of BiasTokens.</summary>
+    public ReadOnlySpan<float> BiasValues;
+    /// <summary>Empty: every token is allowed.</summary>
+    public ReadOnlySpan<uint> Mask;
 }

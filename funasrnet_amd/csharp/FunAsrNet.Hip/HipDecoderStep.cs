@@ -10,10 +10,14 @@ public sealed unsafe class HipDecoderStep : IDecoderStep
     private IntPtr _decoder;
     private readonly HipStepBatcher? _batcher;
     private bool _joined;   // registered with the batcher: this decoder is stepping
+    private bool _choosing; // tokens are chosen since the last prefill: this decoder steps on its own
 
-    private HipDecoderStep(IntPtr decoder, HipStepBatcher? batcher)
+    private readonly int _vocab;
+
+    private HipDecoderStep(IntPtr decoder, int vocab, HipStepBatcher? batcher)
     {
         _decoder = decoder;
+        _vocab = vocab;
         _batcher = batcher;
         _batcher?.AddUser();
     }
@@ -136,7 +140,7 @@ public sealed unsafe class HipDecoderStep : IDecoderStep
                     throw;
                 }
             }
-            return new HipDecoderStep(decoder, batcher);
+            return new HipDecoderStep(decoder, config.Vocab, batcher);
         }
         finally
         {
@@ -152,7 +156,7 @@ public sealed unsafe class HipDecoderStep : IDecoderStep
     internal HipDecoderStep CreateSession(int capacity)
     {
         Native.Check(Native.fah_decoder_create_session(Handle, capacity, out var session));
-        return new HipDecoderStep(session, _batcher);
+        return new HipDecoderStep(session, _vocab, _batcher);
     }
 
     public int Position
@@ -167,6 +171,7 @@ public sealed unsafe class HipDecoderStep : IDecoderStep
     public void SetPosition(int position)
     {
         Leave();
+        _choosing = false;
         Native.Check(Native.fah_decoder_set_position(Handle, position));
     }
 
@@ -175,6 +180,7 @@ public sealed unsafe class HipDecoderStep : IDecoderStep
         if (frames > 1)
         {
             Leave();   // a prefill: the next request's first step joins again
+            _choosing = false;
         }
         fixed (float* x = embeddings) fixed (float* y = logits)
         {
@@ -185,10 +191,10 @@ public sealed unsafe class HipDecoderStep : IDecoderStep
     /// <summary>Greedy -> Embed -> Decode(1) (FunAsr.cs:167-178). With a batcher the
     /// decoder joins it at its first step after a prefill, so the collecting thread
     /// waits only for decoders that are stepping; a decoder whose next position is
-    /// past the batcher's bound steps on its own.</summary>
+    /// past the batcher's bound, or whose tokens are chosen, steps on its own.</summary>
     public int NextToken()
     {
-        if (_batcher is not null && Position < _batcher.MaxPositions)
+        if (_batcher is not null && !_choosing && Position < _batcher.MaxPositions)
         {
             if (!_joined)
             {
@@ -199,6 +205,35 @@ public sealed unsafe class HipDecoderStep : IDecoderStep
         }
         int token;
         Native.Check(Native.fah_decoder_generate(Handle, 1, &token));
+        return token;
+    }
+
+    /// <summary>fah_decoder_choose. The decoder leaves the batcher until the next
+    /// prefill, because lock-step steps keep no logits.</summary>
+    public int Choose(TokenRules rules, float[]? logits)
+    {
+        if (rules.BiasTokens.Length != rules.BiasValues.Length)
+        {
+            throw new ArgumentException("a bias value for each bias token");
+        }
+        if (!rules.Mask.IsEmpty && rules.Mask.Length < (_vocab + 31) / 32)
+        {
+            throw new ArgumentException("a mask bit for each token");
+        }
+        if (logits is not null && logits.Length < _vocab)
+        {
+            throw new ArgumentException("logits for each token");
+        }
+        Leave();
+        _choosing = true;
+        int token;
+        fixed (int* history = rules.History, biasTokens = rules.BiasTokens)
+        fixed (float* biasValues = rules.BiasValues, y = logits)
+        fixed (uint* mask = rules.Mask)
+        {
+            Native.Check(Native.fah_decoder_choose(Handle, history, rules.History.Length, rules.PromptCount,
+                rules.Repetition == 0 ? 1 : rules.Repetition, rules.Presence, rules.Frequency, biasTokens, biasValues, rules.BiasTokens.Length, mask, y, out token));
+        }
         return token;
     }
 

@@ -1,6 +1,7 @@
 """Refusals and sizes of the serving operators that need no device: the
 *_workspace calls check a descriptor as the device calls do."""
 import ctypes
+import os
 from types import SimpleNamespace
 
 import numpy as np
@@ -141,3 +142,12 @@ def test_choose_arguments(monkeypatch):
             decoder.choose(**bad)
     assert not seen and np.all(fixed == 0)
     decoder.handle = None  # nothing to destroy
+
+
+def test_choose_is_reached_from_csharp():
+    """The binding's import has a caller, which the core's interface names."""
+    folder = os.path.join(os.path.dirname(hip.__file__), "csharp")
+    step = open(os.path.join(folder, "FunAsrNet.Hip", "HipDecoderStep.cs")).read()
+    core = open(os.path.join(folder, "FunAsrNet.CorePatch", "IDecoderStepBackend.cs")).read()
+    assert "Native.fah_decoder_choose(Handle" in step and "public int Choose(TokenRules rules, float[]? logits)" in step
+    assert "int Choose(TokenRules rules, float[]? logits);" in core
