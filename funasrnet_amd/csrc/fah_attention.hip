@@ -113,7 +113,8 @@ struct Task {
 };
 
 // Where it goes: the finished rows, or partial ones for a join: sums and total
-// of the weights 2^(c (s - mark) + kLift), and the mark, a score q k.
+// of the weights 2^(c (s - mark) + kLift), and the mark, a score in units of
+// mark_unit.
 template <typename Q>
 struct Sink {
   Q* out;                    // token 0, the K/V head's first query head; null: partial
@@ -121,6 +122,12 @@ struct Sink {
   float* sums;               // [rows][D]
   float* marks;              // [rows][2]
 };
+
+// Marks are scores q k times the scale's power of two: exact, and neither too
+// large nor too small where the scaled scores are not. What is left of the scale,
+// as exponents of two, is mark_exponent.
+__device__ __forceinline__ float mark_unit(float scale) { return fmaxf(u2f(f2u(scale) & 0x7f800000u), 0x1p-126f); }
+__device__ __forceinline__ float mark_exponent(float scale) { return scale / mark_unit(scale) * kLog2e; }
 
 template <int D>
 struct Tile {
@@ -238,10 +245,10 @@ struct SlowRow {
 
 // A row by one wave, only keys that it sees read: all channels, or those that
 // infinite or NaN values between `masked` and `last` can have reached, which the
-// row's tiles masked or took in two parts. A key a lane
-// for the scores, two channels a lane for the values; over once every channel
-// asked for is NaN. (24 prompts of 5014 rows, fp16, every value NaN: 1.3 ms, 12
-// key by key; one channel infinite everywhere 5.4; the first key alone 0.1.)
+// row's tiles masked or took in two parts. A key a lane for the scores, two
+// channels a lane for the values; over once every channel asked for is NaN. (24
+// prompts of 5014 rows, fp16, every value NaN: 1.1 ms, 12 key by key; one channel
+// infinite everywhere 5.4; the first key alone 0.1.)
 template <typename Q, typename K>
 __device__ __noinline__ SlowRow slow_row(const Q* q, const K* k_rows, const K* v_rows, unsigned k_row, unsigned v_row, int begin,
                                          int lim, bool all, int masked, int last, int size, float scale) {
@@ -256,7 +263,7 @@ __device__ __noinline__ SlowRow slow_row(const Q* q, const K* k_rows, const K* v
     if (__builtin_amdgcn_ballot_w64(holds && !(bad[0] && bad[1])) == 0) break;
   }
   if (__builtin_amdgcn_ballot_w64(bad[0] || bad[1]) == 0) return {};
-  const float c = scale * kLog2e;
+  const float unit = mark_unit(scale), c = mark_exponent(scale);
   float sum[2] = {}, top = -kInf, total = 0.0f;
   for (int first = begin; first < lim; first += 64) {
     const int n = lim - first < 64 ? lim - first : 64;
@@ -266,7 +273,7 @@ __device__ __noinline__ SlowRow slow_row(const Q* q, const K* k_rows, const K* v
       alignas(16) K part[8];
       *reinterpret_cast<uint4*>(part) = *reinterpret_cast<const uint4*>(k + e);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += (float)q[e + i] * (float)part[i];
+      for (int i = 0; i < 8; ++i) s += (float)q[e + i] * unit * (float)part[i];
     }
     if (lane >= n) s = -kInf;
     float next = fmaxf(top, s);  // (NaN scores make the total NaN below)
@@ -608,6 +615,7 @@ struct Core {
     }
     total += other_half(total);
     const float unit = __builtin_amdgcn_exp2f(-over(ref, ref_c));  // sums to those of the mark
+    const float to_mark = fminf(fmaxf(unlift * mark_unit(scale), 0x1p-126f), 0x1p127f);
 
     // The last key that a tile with masked places can have held.
     const int tiles_end = t.begin + (end - t.begin + TR - 1) / TR * TR, masked_last = tiles_end <= last ? tiles_end - 1 : last;
@@ -652,7 +660,7 @@ struct Core {
               *reinterpret_cast<f32x4*>(dst + 32 * i + 8 * j) =
                   f32x4{acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]} * factor;
           if (half == 0) {
-            sink.marks[2 * my_row] = ref * unlift;
+            sink.marks[2 * my_row] = ref * to_mark;
             sink.marks[2 * my_row + 1] = total * factor;
           }
         }
@@ -703,7 +711,7 @@ struct Core {
       factor = weight(ref) * unit * (sink.out ? sum == 0.0f ? 0.0f : 1.0f / sum : 1.0f);
     }
     if (half == 0 && wk == 0) {
-      marks[64 * kWaves + my_row * 2] = top * unlift;
+      marks[64 * kWaves + my_row * 2] = top * to_mark;
       marks[64 * kWaves + my_row * 2 + 1] = sum;
     }
     // A share that saw nothing is zeros, also where its values are not finite.
@@ -935,7 +943,7 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void packed_kernel(fah_packed_atte
 template <int D>
 struct Joined {
   static constexpr int kLanes = D / 4;
-  float c;                           // exponents of two a score
+  float c;                           // mark_exponent
   float top = -kInf, total = 0.0f;   // the mark of what is joined so far
   f32x4 o = {};
   template <typename At, typename Marks>
@@ -998,7 +1006,7 @@ __global__ __launch_bounds__(kThreads) void packed_join_kernel(fah_packed_attent
   const int shares = shares_of(visible_keys(p, group), cut);
   if (shares == 1) return;
   const float* sums = static_cast<const float*>(a.workspace) + ((size_t)slot * a.kv_heads + head) * cut.splits * BM * (D + 2);
-  Joined<D> j{a.scale * kLog2e};
+  Joined<D> j{mark_exponent(a.scale)};
   j.add(shares, [&](int i) { return sums + (size_t)i * BM * (D + 2) + r * D + 4 * chunk; },
         [&](int i) { return sums + (size_t)i * BM * (D + 2) + BM * D + 2 * r; });
   const int row = p.row0 + r;
@@ -1105,7 +1113,7 @@ __global__ __launch_bounds__(kThreads) void prefix_join_kernel(fah_prefix_attent
   const size_t first = (size_t)head * shares * all + s * group + g;
   const size_t own = cut.prefix_rows + ((size_t)s * a.kv_heads + head) * cut.own_shares * group + g;
   auto row = [&](int i) { return i < shares ? first + (size_t)i * all : own + (size_t)(i - shares) * group; };
-  Joined<D> j{a.scale * kLog2e};
+  Joined<D> j{mark_exponent(a.scale)};
   j.add(shares + cut.own_shares, [&](int i) { return sums + row(i) * D; }, [&](int i) { return marks + 2 * row(i); });
   if (4 * chunk < a.head_size) j.write(static_cast<Q*>(a.output) + s * a.output_sequence + q_head * a.output_head + 4 * chunk);
 }

@@ -26,8 +26,12 @@ struct alignas(16) Vec {
 };
 
 // 16 bytes past the caches: adjusted logits are not read again here, and would
-// push the rows to come out of them (256 rows of 151936 in bf16: 33.4 us,
-// 47.5 with plain stores; with loads past them as well 39).
+// push the rows to come out of them. 256 rows of 151936 in bf16: 33.5 us where the
+// inputs are in the 256 MB cache (34.7 with plain stores, 39 with loads past the
+// caches as well), 41 where they are not (42.4). 64 rows in fp32 18.9 and 24.4
+// (20, 26.3), 16 rows 11 (11.7), one row 7.5 either way. Whoever reads the adjusted
+// logits next pays for it: a call and a copy of them 61.5 and 68.5 us for 256 rows
+// (57.3, 70), 35.7 and 39.5 for 64 (32.2, 36.8), 16.6 for 16 (15.9 to 17.7).
 template <typename T>
 __device__ __forceinline__ void stream_out(T* p, const Vec<T>& v) {
   using Bits = __attribute__((ext_vector_type(4))) unsigned;

@@ -1062,6 +1062,54 @@ def test_scores_whose_differences_are_their_last_bits(backend, types, powers, or
             check_exact_scores(got[s:s + 1], q[s:s + 1], k[:2000 + n], v[:2000 + n], 2000 + n, types, scale, 12 * unit)
 
 
+@pytest.mark.parametrize("magnitude,scale", [(1e36, 1e-38), (1e30, 1e-31), (1e-6, 1e5), (1e-30, 1e29), (1e-37, 1e36)])
+def test_shares_of_fp32_queries_of_any_size(backend, magnitude, scale):
+    """Joined rows whose scores before scaling are beyond 32 bits, or close to nothing."""
+    types, f = ("f32", "f16"), np.float32(scale)
+    q, k, v = packed_inputs(14, [60, 3], [2100, 1300], 4, 2, 128, types)
+    q *= np.float32(magnitude)
+    k = store(load(k, "f16") * 40, "f16") if magnitude > 1e30 else k
+    qo, ko = offsets([60, 3]), offsets([2100, 1300])
+    check_packed(run_packed(backend, q, k, v, qo, ko, types, scale=float(f)), q, k, v, qo, ko, types, scale=float(f))
+    lengths = [3, 400, 0, 77]
+    q, pk, pv, k, v = prefix_inputs(15, 4, 1500, 400, 4, 2, 128, types)
+    q *= np.float32(magnitude)
+    pk, k = (store(load(x, "f16") * 40, "f16") if magnitude > 1e30 else x for x in (pk, k))
+    for heads_first in (True, False):
+        got = run_prefix(backend, q, pk, pv, k, v, lengths, types, scale=float(f), heads_first=heads_first)
+        check_prefix(got, q, pk, pv, k, v, lengths, types, scale=float(f))
+    # A value that is not finite, where rows are formed again.
+    v[1, 399, 1] = np.inf
+    got = run_prefix(backend, q, pk, pv, k, v, lengths, types, scale=float(f))
+    assert np.all(got[1, 2:] == np.inf)
+    check_prefix(got[[0, 2, 3]], q[[0, 2, 3]], pk, pv, k[[0, 2, 3]], v[[0, 2, 3]], [3, 0, 77], types, scale=float(f))
+
+
+def test_calls_without_any_keys(backend):
+    """No key rows at all, and their buffers NULL: zeros."""
+    from funasrnet_amd import hip
+    rng = np.random.default_rng(2)
+    for kinds, dtype in ((("f32", "f16"), np.float32), (("f16", "f16"), np.float16), (("bf16", "bf16"), np.uint16)):
+        q = to_device(store(rng.standard_normal((9, 4, 64)), kinds[0]))
+        assert q.dtype == dtype
+        codes = dict(query_type=CODES[kinds[0]], cache_type=CODES[kinds[1]], scale=0.125, heads=4, kv_heads=2, head_size=64)
+        zero, at = to_device(np.zeros(10, np.int32)), to_device(np.array([0, 4, 9], np.int32))
+        out = to_device(np.full((9, 4, 64), 3, dtype))
+        call = hip.PackedAttention(query=q.ptr, output=out.ptr, query_row=256, query_head=64, key_row=128, key_head=64, value_row=128,
+                                   value_head=64, output_row=256, output_head=64, query_offsets=at.ptr, key_offsets=zero.ptr,
+                                   sequences=2, query_rows=9, longest_query=5, **codes)
+        assert backend.attention_packed_workspace(call) == 0 and backend.attention_packed_device(call) == hip.OK
+        backend.synchronize()
+        assert np.all(load(out.numpy(), kinds[0]) == 0)
+        out = to_device(np.full((9, 4, 64), 3, dtype))
+        call = hip.PrefixAttention(query=q.ptr, output=out.ptr, lengths=zero.ptr, query_sequence=256, query_head=64, prefix_key_row=64,
+                                   prefix_value_row=64, key_row=64, value_row=64, output_sequence=256, output_head=64, sequences=9,
+                                   **codes)
+        assert backend.attention_prefix_workspace(call) == 0 and backend.attention_prefix_device(call) == hip.OK
+        backend.synchronize()
+        assert np.all(load(out.numpy(), kinds[0]) == 0)
+
+
 @pytest.mark.parametrize("power", [126, 118, -112])
 @pytest.mark.parametrize("queries,keys,heads,kv_heads,size", [(130, 130, 4, 2, 128), (1100, 1100, 64, 64, 64), (9, 3000, 4, 2, 128)],
                          ids=str)
