@@ -232,7 +232,8 @@ public sealed unsafe class HipDecoderStep : IDecoderStep
         fixed (uint* mask = rules.Mask)
         {
             Native.Check(Native.fah_decoder_choose(Handle, history, rules.History.Length, rules.PromptCount,
-                rules.Repetition == 0 ? 1 : rules.Repetition, rules.Presence, rules.Frequency, biasTokens, biasValues, rules.BiasTokens.Length, mask, y, out token));
+                rules.Repetition == 0 ? 1 : rules.Repetition, rules.Presence, rules.Frequency, biasTokens, biasValues,
+                rules.BiasTokens.Length, mask, y, out token));
         }
         return token;
     }

@@ -288,8 +288,11 @@ enum { FAH_TYPE_F32 = 0, FAH_TYPE_F16 = 1, FAH_TYPE_BF16 = 2 };
  * key_offsets[s + 1]; its last query sees its last key, so with Lq queries and
  * Lk keys query i sees the keys j <= i + Lk - Lq (Lk > Lq: the first Lk - Lq
  * rows were cached before). Per query head h, with K/V head h / (heads /
- * kv_heads): softmax(scale q k) over the keys seen, times their values, in
- * 32-bit sums. A query that sees no key (Lk < Lq, or none at all), or whose
+ * kv_heads): softmax(scale q k) over the keys seen, times their values. Scores,
+ * totals and sums are 32-bit; the softmax's weights are rounded once to the
+ * cache's type for the products with the values where queries are 16-bit, and
+ * held in 22 bits for fp32 queries, which themselves count to 22 bits. A query
+ * that sees no key (Lk < Lq, or none at all), or whose
  * every score is -infinity, gets zeros. Keys and values that a query does not
  * see never reach its output, whatever they hold. Output rows of no sequence
  * are left as they were. */
@@ -312,7 +315,9 @@ typedef struct fah_packed_attention {
 
 /* Declines head sizes that are no multiple of 8 or above 128, more than 65536
  * heads, other pairs of types, rows that do not start on 16 bytes (addresses and
- * strides), and key or value rows more than 2^25 elements apart. */
+ * strides), and key or value rows more than 2^25 elements apart. More than
+ * 2^31 - 2^19 - 1 keys, 2^30 - 1 query rows times heads or 2^23 - 1 sequences times
+ * heads are errors. */
 int fah_attention_packed_device(fah_context* context, const fah_packed_attention* call);
 int fah_attention_packed_workspace(const fah_packed_attention* call, int64_t* bytes);
 
@@ -320,8 +325,8 @@ int fah_attention_packed_workspace(const fah_packed_attention* call, int64_t* by
  * their first `prefix` keys and values (one copy, read once for all; the
  * device-side form of what CachePrefix and RestorePrefix keep per decoder,
  * src/FunAsrNet/QwenDecoder.cs:122-137), followed by each sequence's own
- * lengths[s] cache rows: softmax over both together, in 32-bit sums, heads
- * grouped as in fah_packed_attention. prefix 0 is attention over the own rows
+ * lengths[s] cache rows: softmax over both together, heads grouped and values
+ * rounded as in fah_packed_attention. prefix 0 is attention over the own rows
  * alone. A token that sees no key, or whose every score is -infinity, gets
  * zeros. Cache rows from lengths[s] on are not read. */
 typedef struct fah_prefix_attention {
