@@ -240,9 +240,9 @@ struct Ctx {
 // persistent section holds the lock from before its launches until its
 // stream has drained, after making its stream wait for the work already
 // enqueued on the other contexts' streams: no call of another context can
-// then put a kernel beside it. (Graphs that a caller replays and work that was
-// under way on a stream when its capture began are not waited for: kernels that
-// end leave the step its CUs, which it waits for.)
+// then put a kernel beside it. (Graphs that a caller launches meanwhile and work
+// that was under way on a stream when its capture began are not waited for:
+// kernels that end leave the step its CUs, which it waits for.)
 struct DeviceGate {
   std::mutex m;
   std::vector<Ctx*> members;

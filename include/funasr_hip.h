@@ -24,8 +24,8 @@
  * every CU of the device) first waits for the work already enqueued by the
  * other contexts and keeps the device to itself until it has finished: calls
  * of other contexts that enqueue wait until then, and no kernel of theirs runs
- * beside it. It does not see graphs that a caller replays, nor a stream under
- * capture.
+ * beside it. It does not see graphs that a caller launches meanwhile or on
+ * streams of its own, nor what a stream under capture still had to run.
  *
  * Lifetime: weights and decoders keep their context's state alive.
  * fah_context_destroy releases the handle (which must not be used again);
@@ -270,13 +270,14 @@ int fah_q8_block_dots_device(fah_context* context, const int8_t* q, const fah_we
  * other streams with it through fah_context_stream and events); the calls
  * copy nothing, wait for no work of their stream, allocate nothing and keep
  * nothing, so they may be captured into graphs, also while other contexts run
- * decoder steps. (A call may have to wait until another context's persistent
- * step has ended, as above.) What they need beyond their outputs is the
- * caller's `workspace`: at least the bytes that the *_workspace call of the
- * same descriptor gives (it needs no device and reads nothing through the
- * pointers), 16-byte aligned, its contents free before and after. Calls that
- * may run at the same time, such as two graphs replayed on different streams,
- * need workspaces of their own.
+ * decoder steps (which may allocate: capture in a mode that lets other threads
+ * do so, thread-local or relaxed). A call may have to wait until another
+ * context's persistent step has ended, as above. What they need beyond their
+ * outputs is the caller's `workspace`: at least the bytes that the *_workspace
+ * call of the same descriptor gives (it needs no device and reads nothing
+ * through the pointers), 16-byte aligned, its contents free before and after.
+ * Calls that may run at the same time, such as two graphs replayed on different
+ * streams, need workspaces of their own.
  * No output may overlap an input or the workspace unless its comment says so. */
 
 /* Element types. */
@@ -292,10 +293,9 @@ enum { FAH_TYPE_F32 = 0, FAH_TYPE_F16 = 1, FAH_TYPE_BF16 = 2 };
  * totals and sums are 32-bit; the softmax's weights are rounded once to the
  * cache's type for the products with the values where queries are 16-bit, and
  * held in 22 bits for fp32 queries, which themselves count to 22 bits. A query
- * that sees no key (Lk < Lq, or none at all), or whose
- * every score is -infinity, gets zeros. Keys and values that a query does not
- * see never reach its output, whatever they hold. Output rows of no sequence
- * are left as they were. */
+ * that sees no key (Lk < Lq, or none at all), or whose every score is -infinity,
+ * gets zeros. Keys and values that a query does not see never reach its output,
+ * whatever they hold. Output rows of no sequence are left as they were. */
 typedef struct fah_packed_attention {
     const void* query;  /* [query_rows][heads][head_size] */
     const void* key;    /* [key_rows][kv_heads][head_size] */
